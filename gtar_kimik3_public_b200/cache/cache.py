@@ -13,7 +13,8 @@ fixed size per batch row (src/cache.py:48-57).  Here
   pool of its own: one group for "all positions", one per window length (pages that have left
   the window go back to the pool, except those of first positions that the request keeps), one per
   shape of fixed-size state; a group's pages hold keys and values per kv head (values may have a width
-  of their own), or one row per position for all heads (a layer that attends through a latent);
+  of their own), or one row per position for all heads (a layer that attends through a latent); a request may
+  ask for keys and values in 8 bits (e4m3 numbers and a byte, the power of two of the row, per position and kv head);
 * stale data is never cleared from pages: nothing reads beyond a sequence's length (the
   reference argues the same for its rollback, src/cache.py:37-45).  State rows are zeroed when
   a slot is handed out.
@@ -28,7 +29,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from ..ops.functional import DecodeWork, PagedKV, PagedRows
+from ..ops.functional import DecodeWork, PagedKV, PagedKV8, PagedRows, Work8
 from ..parts.base import KVRequest, RowsRequest, StateRequest
 from .allocators import CacheFull, PageAllocator, SlotAllocator
 
@@ -68,6 +69,12 @@ class _KVGroup:
         if isinstance(request, RowsRequest):  # one row per position; no second tensor
             self.k = torch.empty((len(items), n_pages, page_size, request.width), dtype=dtype, device=device)
             self.v = None
+        elif request.dtype is not None:
+            if request.dtype != torch.float8_e4m3fn or request.value_dim not in (None, request.head_dim):
+                raise ValueError(f"a cache keeps keys and values of one size in float8_e4m3fn, not {request}")
+            shape = (len(items), n_pages, request.n_kv_heads, page_size)
+            self.k, self.v = (torch.empty((*shape, request.head_dim), dtype=request.dtype, device=device) for _ in range(2))
+            self.k_exp, self.v_exp = (torch.empty(shape, dtype=torch.uint8, device=device) for _ in range(2))
         else:
             shape = (len(items), n_pages, request.n_kv_heads, page_size)
             self.k = torch.empty((*shape, request.head_dim), dtype=dtype, device=device)
@@ -80,7 +87,8 @@ class _KVGroup:
         self.upto: dict[int, int] = {}  # slot -> one past the highest page index the sequence ever had
         self.dirty: set[int] = set()
         self._staging = None  # pinned copies of the table for uploads, made at the first upload
-        self._work = None  # decode attention's scratch for this group's layers, made with the first view
+        self._work = None  # attention's scratch for this group's layers, made with the first view
+        self._views: dict[tuple[int, int], PagedKV8] = {}
 
     def open_slot(self, slot: int) -> None:
         self.owned[slot] = {}
@@ -158,8 +166,14 @@ class _KVGroup:
         self._staging_events[turn] = event
         self.dirty.clear()
 
-    def view(self, item: tuple[int, int]) -> PagedKV | PagedRows:
+    def view(self, item: tuple[int, int]) -> PagedKV | PagedKV8 | PagedRows:
         i = self.index_of[item]
+        if isinstance(self.request, KVRequest) and self.request.dtype is not None:
+            if item not in self._views:
+                if self._work is None:
+                    self._work = Work8(self.table.device)
+                self._views[item] = PagedKV8(self.k[i], self.v[i], self.k_exp[i], self.v_exp[i], self.table, self._work)
+            return self._views[item]
         if self.v is None:
             return PagedRows(self.k[i], self.table)
         if self._work is None and self.table.is_cuda:
@@ -274,7 +288,7 @@ class Cache:
 
     # ------------------------------------------------------------------ views
     def view(self, entry: int):
-        """Storage of run-list entry ``entry``: a ``PagedKV`` or a state tensor ``[n_slots, ...]`` for a single
+        """Storage of run-list entry ``entry``: a ``PagedKV`` (or ``PagedKV8``) or a state tensor ``[n_slots, ...]`` for a single
         request, None for none, and for a list of requests a tuple of those in the list's order."""
         source = self.layout.shared_with.get(entry, entry)
         request = self.layout.requests[source]
@@ -296,6 +310,8 @@ class Cache:
             r = group.request
             if isinstance(r, RowsRequest):
                 total += len(group.items) * r.width * self.k_element_size()
+            elif r.dtype is not None:
+                total += len(group.items) * r.n_kv_heads * 2 * (r.head_dim + 1)
             else:
                 total += len(group.items) * r.n_kv_heads * (r.head_dim + (r.value_dim or r.head_dim)) * self.k_element_size()
         return total

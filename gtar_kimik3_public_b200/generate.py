@@ -35,14 +35,24 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype must be bfloat16 or float32, got {name!r}") from None
 
 
+def parse_cache_dtype(name) -> torch.dtype | None:
+    """None or "auto": the run's type; "float8_e4m3fn": 8 bits."""
+    if name in (None, "auto"):
+        return None
+    if name in ("float8_e4m3fn", torch.float8_e4m3fn):
+        return torch.float8_e4m3fn
+    raise ValueError(f"cache_dtype must be auto or float8_e4m3fn, got {name!r}")
+
+
 def load(model_dir: str | Path, dtype="bfloat16", device: str | torch.device = "cuda:0",
-         cast_matrices: bool = False) -> Model:
+         cast_matrices: bool = False, cache_dtype=None) -> Model:
     """Builds the model class that ``model_dir/config.json`` names and loads its safetensors.
     ``cast_matrices``: in a bfloat16 run, round matrices that the file stores in 32-bit to bfloat16
-    (by default they stay 32-bit and their projections run on the slow, exact 32-bit kernel)."""
+    (by default they stay 32-bit and their projections run on the slow, exact 32-bit kernel).
+    ``cache_dtype``: "float8_e4m3fn" keeps keys and values in 8 bits (for models whose layers are grouped-query attention)."""
     config = config_from_file(model_dir)
     arch = architecture(config.ARCH_NAMES[0])
-    model = Model(arch.build_plan(config), config, parse_dtype(dtype), device)
+    model = Model(arch.build_plan(config), config, parse_dtype(dtype), device, parse_cache_dtype(cache_dtype))
     load_weights(model, model_dir, cast_matrices=cast_matrices)
     return model
 

@@ -9,13 +9,13 @@ an entry read the storage that an earlier entry writes.
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import torch
 
 from ..cache import Cache, CacheLayout
 from ..ops import functional as F
-from ..parts.base import Block, Norm, Part, PositionEncoding, StepContext, TensorSpec
+from ..parts.base import Block, KVRequest, Norm, Part, PositionEncoding, RowsRequest, StepContext, TensorSpec
 from ..parts.embedding import OutputHead, TokenEmbedding
 
 
@@ -87,9 +87,14 @@ class ModelPlan:
 
 
 class Model:
-    def __init__(self, plan: ModelPlan, config, dtype: torch.dtype, device: torch.device | str):
+    def __init__(self, plan: ModelPlan, config, dtype: torch.dtype, device: torch.device | str, cache_dtype: torch.dtype | None = None):
+        """``cache_dtype``: None keeps keys and values in the run's type, ``torch.float8_e4m3fn`` in 8 bits (half a bfloat16 cache's memory
+        and traffic); every layer that keeps something per position must be able to."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"a model runs in float32 or bfloat16, not {dtype}")
+        if cache_dtype not in (None, torch.float8_e4m3fn):
+            raise ValueError(f"a cache is kept in the run's type (None) or in torch.float8_e4m3fn, not {cache_dtype}")
+        self.cache_dtype = cache_dtype
         self.plan, self.config, self.dtype, self.device = plan, config, dtype, torch.device(device)
         for position, entry in enumerate(plan.run_list):
             if not 0 <= entry.layer < len(plan.layers):
@@ -99,6 +104,17 @@ class Model:
             if entry.enter is not None and entry.enter.step is not None and (plan.steps is None or not 0 <= entry.enter.step < plan.steps.rows):
                 raise ValueError(f"run-list entry {position} names row {entry.enter.step} of the step table, which has no such row")
         self.vocab_size = plan.head.vocab_size
+        if cache_dtype is not None:
+            self._check_cache8()
+
+    def _check_cache8(self) -> None:
+        """Raises where a layer keeps keys, values or rows per position that it cannot read in 8 bits, or where none keeps any."""
+        items = [(e.layer, item) for e, request in zip(self.plan.run_list, self.cache_layout().requests) if request is not None
+                 for item in (request if isinstance(request, (list, tuple)) else (request,)) if isinstance(item, (KVRequest, RowsRequest))]
+        cannot = sorted({layer for layer, item in items if isinstance(item, RowsRequest) or item.dtype is None})
+        if cannot or not items:
+            what = f"layers {cannot} keep theirs in another form" if items else "this model keeps none"
+            raise ValueError(f"a cache in {self.cache_dtype} is for grouped-query attention over keys and values per position: {what}")
 
     # ------------------------------------------------------------------ weights
     def named_parts(self) -> list[tuple[str, Part]]:
@@ -128,8 +144,15 @@ class Model:
     def cache_layout(self) -> CacheLayout:
         plan = self.plan
         requests = [plan.layers[e.layer].cache_request() for e in plan.run_list]
+        if self.cache_dtype is not None:
+            requests = [self._request8(plan.layers[e.layer], r) for e, r in zip(plan.run_list, requests)]
         shared = {i: e.cache_of for i, e in enumerate(plan.run_list) if e.cache_of is not None}
         return CacheLayout(requests, shared)
+
+    def _request8(self, layer: Block, request):
+        if isinstance(request, (list, tuple)):
+            return [self._request8(layer, r) for r in request]
+        return replace(request, dtype=self.cache_dtype) if isinstance(request, KVRequest) and layer.cache8 else request
 
     def make_cache(self, max_tokens: int, max_seqs: int | None = None) -> Cache:
         max_len = getattr(self.config, "max_position_embeddings", None)

@@ -5,6 +5,8 @@
 * bfloat16, every sequence bringing one token: the split-KV decode kernel;
 * bfloat16 otherwise (prompts, or continuations of several tokens): the flash prefill kernel.
 
+Layers whose keys and values are kept in 8 bits (``PagedKV8``) have their own calls for single tokens and for prompts.
+
 Layers that keep one latent row per position for all heads (``latent_attention`` below): bfloat16 rows whose sizes the
 tensor-core kernel takes go there, prompts and single tokens alike (single-token steps cut into splits); everything else, and
 every float32 run, goes to the exact latent kernel.
@@ -51,10 +53,14 @@ def decode_flat_preferred(ctx, n_kv: int, kv: F.PagedKV) -> bool:
                               F.decode_flat_places(kv.k.shape[3], sms))
 
 
-def paged_attention(q: torch.Tensor, kv: F.PagedKV, ctx, scale: float, window: int = 0, sink: bool = False) -> torch.Tensor:
+def paged_attention(q: torch.Tensor, kv: F.PagedKV | F.PagedKV8, ctx, scale: float, window: int = 0, sink: bool = False) -> torch.Tensor:
     """Causal grouped-query attention of the step's queries ``[n_tokens, n_q, d]`` over each
     sequence's cached keys and values (the new tokens' own are already written).  ``sink``: one more term in the
     softmax's denominator (a key of score 0 without a value)."""
+    if isinstance(kv, F.PagedKV8):
+        if ctx.all_single:
+            return F.attention_decode8(q, kv, ctx.kv_len, ctx.slots, ctx.typical_kv_len or ctx.max_kv_len, scale, window, sink)
+        return F.attention_prefill8(q, kv, ctx.cu_q, ctx.kv_len, ctx.slots, ctx.max_q_len, ctx.max_kv_len, scale, window, sink)
     n_q, d = q.shape[1], q.shape[2]
     n_kv = kv.k.shape[1]
     fast = q.dtype == torch.bfloat16 and d in FAST_HEAD_DIMS and kv.page_size == 64 and n_q // n_kv <= 16

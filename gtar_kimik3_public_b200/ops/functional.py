@@ -7,6 +7,7 @@ output.  Shapes follow the packed ("varlen") convention of the step function: ac
 
 from __future__ import annotations
 
+import ctypes
 import functools
 from dataclasses import dataclass
 
@@ -334,6 +335,9 @@ def attention_exact(
 _error_flags: dict[int, torch.Tensor] = {}
 
 
+ERR_PLACE8 = 80  # cache8::ERR_PLACE
+
+
 def error_flag(device: torch.device) -> torch.Tensor:
     """The device int that kernels with bounded waits set when a wait gives up (0 = all well)."""
     index = device.index if device.index is not None else torch.cuda.current_device()
@@ -348,6 +352,8 @@ def check_kernel_errors(device: torch.device | str = "cuda:0") -> None:
     code = int(flag.item())
     if code:
         flag.zero_()
+        if code == ERR_PLACE8:
+            raise KernelError("a call over 8-bit pages met a page number, slot, sequence, position or length outside its pools; its output is not valid")
         raise KernelError(f"a kernel gave up waiting on a barrier (code {code}); its output is not valid")
 
 
@@ -2418,3 +2424,182 @@ def memory_chunked(proj: torch.Tensor, at: MemoryColumns, gate_bias: torch.Tenso
          ptr(n_state), ptr(norm_w), float(eps), ptr(y), ptr(states), ptr(scalars), ptr(start), ptr(cu_q), ptr(slots), int(n_seqs), H, d, dv,
          int(max_q_len), wave, stream_ptr())
     return y
+
+
+# ------------------------------------------------------------------ the 8-bit cache
+class _Pages8(ctypes.Structure):
+    """The kernels' description of one layer's 8-bit pages (``GkPages8`` in csrc/cache8.cuh)."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("error", ctypes.c_void_p), ("n_pages", ctypes.c_longlong), ("n_slots", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("n_kv", ctypes.c_int), ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+CACHE8_MAX_HEAD_DIM = 512
+
+
+@dataclass(frozen=True, eq=False)
+class PagedKV8:
+    """One layer's keys and values in pages of 8-bit numbers, and the table that maps a sequence's pages.
+
+    ``k``, ``v``: ``[n_pages, n_kv_heads, page_size, head_dim]`` float8_e4m3fn; ``k_exp``, ``v_exp``: ``[n_pages, n_kv_heads, page_size]`` uint8,
+    the power of two of each row plus 127: a number is ``k * 2 ** (k_exp - 127)``, exact in bfloat16.  The power is the smallest for which
+    the row's largest finite number stays within 448, kept within -64 .. 119.  What is not finite is kept as NaN.  ``block_table``:
+    ``[n_slots, max_pages]`` int32.  Page numbers, slots and lengths that lie outside these are skipped by the kernels and
+    recorded for ``check_kernel_errors``.  The tensors are looked at once, here: a view stands for the same memory as long as it lives.
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: torch.Tensor
+    v_exp: torch.Tensor
+    block_table: torch.Tensor
+    work: "Work8 | None" = None  # what attention keeps between launches; the cache group owns it
+
+    def __post_init__(self):
+        require_device(self.k.device)
+        for name, t, dtype, dims in (("k pages", self.k, torch.float8_e4m3fn, 4), ("v pages", self.v, torch.float8_e4m3fn, 4),
+                                     ("k exponents", self.k_exp, torch.uint8, 3), ("v exponents", self.v_exp, torch.uint8, 3),
+                                     ("block_table", self.block_table, torch.int32, 2)):
+            _check(t, name, dtype, dims)
+            if t.device != self.k.device:
+                raise KernelError(f"{name} are on {t.device}, k pages on {self.k.device}")
+        n_pages, n_kv, page, d = self.k.shape
+        if self.v.shape != self.k.shape:
+            raise KernelError(f"8-bit pages of keys {tuple(self.k.shape)} and of values {tuple(self.v.shape)} must be alike")
+        if self.k_exp.shape != self.k.shape[:3] or self.v_exp.shape != self.k.shape[:3]:
+            raise KernelError(f"exponents must be {tuple(self.k.shape[:3])}, got {tuple(self.k_exp.shape)} and {tuple(self.v_exp.shape)}")
+        if page % 32 or d % 2 or not 0 < d <= CACHE8_MAX_HEAD_DIM:
+            raise KernelError(f"8-bit pages take a page size that is a multiple of 32 and an even head size up to {CACHE8_MAX_HEAD_DIM}, got {page} and {d}")
+        if self.work is None:
+            object.__setattr__(self, "work", Work8(self.k.device))
+        pages = _Pages8(ptr(self.k), ptr(self.v), ptr(self.k_exp), ptr(self.v_exp), ptr(self.block_table), ptr(error_flag(self.k.device)), n_pages,
+                        self.block_table.shape[0], self.block_table.shape[1], n_kv, page, d)
+        object.__setattr__(self, "_pages", pages)
+        object.__setattr__(self, "_at", ctypes.addressof(pages))
+
+    @property
+    def page_size(self) -> int:
+        return self.k.shape[2]
+
+    @property
+    def max_pages(self) -> int:
+        return self.block_table.shape[1]
+
+
+class Work8:
+    """Memory that attention over 8-bit pages keeps between launches, one per cache group (its layers run one after another on one stream)."""
+
+    def __init__(self, device: torch.device):
+        self.device = device
+
+
+def _check8(kv: PagedKV8, given: torch.Tensor, *ints: tuple[str, torch.Tensor, int]) -> None:
+    """What every call over 8-bit pages asks of its tensors: ``ints`` are (name, int32 tensor, entries or -1)."""
+    device = kv.k.device
+    if given.device != device:
+        raise KernelError(f"the tensors are on {given.device}, the pages on {device}")
+    if device.index != torch.cuda.current_device():
+        raise KernelError(f"the pages are on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+    for name, t, entries in ints:
+        if t.dtype != torch.int32 or t.dim() != 1 or t.device != device or not t.is_contiguous():
+            raise KernelError(f"{name} must be a contiguous int32 vector on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if entries >= 0 and t.shape[0] != entries:
+            raise KernelError(f"{name} must have {entries} entries, got {t.shape[0]}")
+
+
+def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float,
+                        cos: torch.Tensor | None, sin: torch.Tensor | None, tok_pos: torch.Tensor, tok_seq: torch.Tensor, slots: torch.Tensor,
+                        kv: PagedKV8, max_position: int, q_out: torch.Tensor | None = None, write_kv: bool = True) -> torch.Tensor:
+    """``qk_norm_rope_write`` into 8-bit pages: per-head RMSNorm of q and k, rotation by position, and the write of k and v as e4m3 numbers
+    with a power of two a (position, kv head) (see ``PagedKV8``).  Everything is 32-bit up to the one rounding of each result.  Returns the
+    queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
+    _check(qkv, "qkv", dims=2)
+    n = qkv.shape[0]
+    _check8(kv, qkv, ("tok_pos", tok_pos, n), ("tok_seq", tok_seq, n), ("slots", slots, -1))
+    code = dtype_code(qkv.dtype)
+    if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
+        raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
+    if kv.k.shape[1] != n_kv or kv.k.shape[3] != head_dim:
+        raise KernelError(f"pages {tuple(kv.k.shape)} do not fit n_kv={n_kv}, head_dim={head_dim}")
+    weight_code = 0
+    if (q_weight is None) != (k_weight is None):
+        raise KernelError("q and k are normed both or neither")
+    if q_weight is not None:
+        _check(q_weight, "q_weight", dims=1)
+        _check(k_weight, "k_weight", q_weight.dtype, 1)
+        if q_weight.shape[0] != head_dim or k_weight.shape[0] != head_dim:
+            raise KernelError("q/k norm weights must have head_dim entries")
+        weight_code = dtype_code(q_weight.dtype)
+    table_positions = 0
+    if (cos is None) != (sin is None):
+        raise KernelError("cos and sin tables go together")
+    if cos is not None:
+        _check(cos, "cos", torch.float32, 2)
+        _check(sin, "sin", torch.float32, 2)
+        if cos.shape[1] != head_dim // 2 or sin.shape != cos.shape:
+            raise KernelError("rotary tables must be [positions, head_dim / 2]")
+        table_positions = cos.shape[0]
+    if q_out is None:
+        q_out = torch.empty((n, n_q, head_dim), dtype=qkv.dtype, device=qkv.device)
+    _check(q_out, "q_out", qkv.dtype, 3)
+    if q_out.shape != (n, n_q, head_dim):
+        raise KernelError(f"q_out is {tuple(q_out.shape)}, expected {(n, n_q, head_dim)}")
+    call("gk_write8", kv._at, ptr(qkv), code, ptr(q_weight), ptr(k_weight), weight_code, int(q_weight is not None), float(eps), ptr(cos), ptr(sin),
+         table_positions, int(max_position), ptr(tok_pos), ptr(tok_seq), ptr(slots), slots.shape[0], ptr(q_out), n, n_q, int(write_kv), stream_ptr())
+    return q_out
+
+
+def read_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, out: PagedKV | None = None, last: int = 0) -> PagedKV:
+    """The 8-bit pages of the listed sequences read back, exactly, as bfloat16 pages of the same numbers: those that hold each sequence's last
+    ``last`` positions (0: all).  Places behind a sequence's end in its last page become zero; pages that the step does not name are left as they
+    were.  ``out``: pages of the same shape (made here if there are none); ``max_kv_len``: the longest of ``kv_len``, known on the host."""
+    n = kv_len.shape[0]
+    _check8(kv, kv_len, ("kv_len", kv_len, n), ("slots", slots, n))
+    if out is None:
+        k, v = (torch.empty(kv.k.shape, dtype=torch.bfloat16, device=kv.k.device) for _ in range(2))
+        out = PagedKV(k, v, kv.block_table)
+    for name, t in (("k pages", out.k), ("v pages", out.v)):
+        _check(t, name, torch.bfloat16, 4)
+        if t.shape != kv.k.shape or t.device != kv.k.device:
+            raise KernelError(f"{name} to read into are {tuple(t.shape)} on {t.device}, expected {tuple(kv.k.shape)} on {kv.k.device}")
+    call("gk_read8", kv._at, ptr(kv_len), ptr(slots), n, int(max_kv_len), int(last), ptr(out.k), ptr(out.v), stream_ptr())
+    return out
+
+
+def _check_queries8(q: torch.Tensor, kv: PagedKV8, out: torch.Tensor | None) -> torch.Tensor:
+    if q.dim() != 3 or not q.is_cuda or not q.is_contiguous():
+        raise KernelError(f"q must be a contiguous CUDA tensor [tokens, heads, head size], got {tuple(q.shape)} on {q.device}")
+    if q.shape[2] != kv.k.shape[3] or q.shape[1] % kv.k.shape[1]:
+        raise KernelError(f"queries {tuple(q.shape)} do not fit pages of {kv.k.shape[1]} kv heads of {kv.k.shape[3]}")
+    if out is None:
+        return torch.empty_like(q)
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise KernelError(f"out must be like q, {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
+    return out
+
+
+def attention_decode8(q: torch.Tensor, kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, scale: float, window: int = 0,
+                      sink: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence (``q [n_seqs, n_q, d]``, bfloat16 or float32) over 8-bit pages; ``kv_len[i]`` counts the sequence's
+    cached tokens including the new one, ``max_kv_len`` is the longest of them or a bound on it.  ``sink``: one more term in the softmax's
+    denominator, a key of score 0 without a value.  A sequence without tokens gets zeros."""
+    out = _check_queries8(q, kv, out)
+    n, n_q, d = q.shape
+    _check8(kv, q, ("kv_len", kv_len, n), ("slots", slots, n))
+    call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), None, ptr(kv_len), ptr(slots), n, n, n_q, float(scale), int(window), int(sink),
+         stream_ptr())
+    return out
+
+
+def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, max_kv_len: int,
+                       scale: float, window: int = 0, sink: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the packed new tokens ``q [n_tokens, n_q, d]`` (bfloat16 or float32) over 8-bit pages.  Sequence ``i`` owns the tokens
+    ``cu_q[i] .. cu_q[i+1]-1``, its last positions: ``kv_len[i]`` counts its cached tokens including them.  ``max_q_len`` and ``max_kv_len`` are the
+    largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were; a token that sees no key gets zeros."""
+    out = _check_queries8(q, kv, out)
+    n_seqs = kv_len.shape[0]
+    _check8(kv, q, ("cu_q", cu_q, n_seqs + 1), ("kv_len", kv_len, n_seqs), ("slots", slots, n_seqs))
+    call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
+         int(window), int(sink), stream_ptr())
+    return out

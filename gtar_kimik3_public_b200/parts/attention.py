@@ -19,6 +19,7 @@ from .base import KVRequest, Mixer, PositionEncoding, StepContext, TensorSpec, r
 
 
 class GQAAttention(Mixer):
+    cache8 = True
     graph_safe = True  # all per-step numbers are read from device memory by the kernels
 
     def __init__(self, hidden_size: int, n_q_heads: int, n_kv_heads: int, head_dim: int, qk_norm_eps: float | None,
@@ -75,7 +76,7 @@ class GQAAttention(Mixer):
                 "qk_dtype": None if self.q_norm is None else self.q_norm.dtype, "rope": rope, "scale": self.scale}
 
     @one_layer
-    def forward(self, x, ctx: StepContext, cache: F.PagedKV) -> torch.Tensor:
+    def forward(self, x, ctx: StepContext, cache: F.PagedKV | F.PagedKV8) -> torch.Tensor:
         cos = sin = None
         if self.position is not None:
             cos, sin = self.position.cos, self.position.sin
@@ -112,10 +113,10 @@ class GQAAttention(Mixer):
     def on_stream_ok(self, h: torch.Tensor, norm_weight, ctx: StepContext, cache) -> bool:
         """Whether ``forward_on_stream`` takes this step: a few tokens, one each, bfloat16 matrices of sizes the
         few-token product takes with the norm inside (see ``ops.linear.linear_on_stream_ok``)."""
-        return (ctx.all_single and ctx.dtype == torch.bfloat16 and isinstance(cache, F.PagedKV)
+        return (ctx.all_single and ctx.dtype == torch.bfloat16 and isinstance(cache, (F.PagedKV, F.PagedKV8))
                 and linear_on_stream_ok(h, norm_weight, self.w_qkv, self.w_o))
 
-    def forward_on_stream(self, h: torch.Tensor, norm_weight: torch.Tensor, norm_eps: float, ctx: StepContext, cache: F.PagedKV) -> None:
+    def forward_on_stream(self, h: torch.Tensor, norm_weight: torch.Tensor, norm_eps: float, ctx: StepContext, cache: F.PagedKV | F.PagedKV8) -> None:
         """``h += attention(rmsnorm(h))`` on the 32-bit stream itself: the norm is formed inside the q|k|v product and
         the add happens in the output product's output stage, so the step has two kernels fewer a layer."""
         cos = sin = None
@@ -128,6 +129,11 @@ class GQAAttention(Mixer):
 
     def _attend(self, qkv: torch.Tensor, ctx: StepContext, cache: F.PagedKV, cos, sin, write_kv: bool) -> torch.Tensor:
         """Attention output ``[n_tokens, n_q, head_dim]`` from the packed projection of the step's tokens."""
+        if isinstance(cache, F.PagedKV8):
+            q = F.qk_norm_rope_write8(
+                qkv, self.n_q, self.n_kv, self.head_dim, self.q_norm, self.k_norm, self.qk_norm_eps or 1.0, cos, sin,
+                ctx.tok_pos, ctx.tok_seq, ctx.slots, cache, ctx.max_position, write_kv=write_kv)
+            return attention_ops.paged_attention(q, cache, ctx, self.scale, self.window or 0)
         if ctx.all_single and attention_ops.fused_decode_ok(qkv, cache, self.n_q, self.n_kv, self.head_dim):
             # one token per sequence: norm, rotation, cache write and attention in one kernel
             if attention_ops.decode_flat_preferred(ctx, self.n_kv, cache):

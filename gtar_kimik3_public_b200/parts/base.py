@@ -52,6 +52,9 @@ class KVRequest:
     window: int | None = None
     value_dim: int | None = None
     keep_first: int = 0
+    # None: kept in the run's type.  torch.float8_e4m3fn: 8 bits and a power of two a (position, kv head); a model's
+    # ``cache_dtype`` puts it here for the mixers that say ``cache8``
+    dtype: torch.dtype | None = None
 
 
 @dataclass(frozen=True)
@@ -136,6 +139,8 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    # Whether ``forward`` takes a ``PagedKV8`` where its ``KVRequest`` has the 8-bit type.
+    cache8 = False
 
     def cache_request(self) -> KVRequest | StateRequest | None | list:
         """What the mixer needs kept between steps: a ``KVRequest``, a ``StateRequest``, None, or a list of
@@ -190,6 +195,11 @@ class Block(Part):
         return bool(parts) and all(part.graph_safe for _, part in parts)
 
     mixer: Mixer
+
+    @property
+    def cache8(self) -> bool:
+        """Whether the keys and values of the layer may be kept in 8 bits."""
+        return getattr(getattr(self, "mixer", None), "cache8", False)
 
     # Whether the block itself adds what stands at its entry of the run list (``ctx.extras["enter"]``) and forms the rows that
     # the next entry's block reads (``ctx.extras["follower"]``); for other blocks the model does the adds.

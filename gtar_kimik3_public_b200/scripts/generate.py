@@ -32,6 +32,8 @@ def build_parser() -> argparse.ArgumentParser:
     parser.add_argument("--checkpoint", help="a checkpoint file of the reference's training loop (its --checkpoint): "
                                              "converted to a model folder first")
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    parser.add_argument("--cache-dtype", default="auto", choices=["auto", "float8_e4m3fn"],
+                        help="what keys and values are kept in: the run's type, or 8 bits")
     parser.add_argument("--cast-matrices", action="store_true",
                         help="bfloat16 run of a folder stored in 32-bit: round its matrices to bfloat16 at load")
     parser.add_argument("--prompt", default=None)
@@ -99,7 +101,8 @@ def main(argv=None) -> int:
             stop_ids.append(eos)
 
     # a checkpoint is 32-bit: as in the reference's engine its matrices are rounded for a bfloat16 run
-    model = load(model_dir, args.dtype, args.device, cast_matrices=args.cast_matrices or bool(args.checkpoint))
+    model = load(model_dir, args.dtype, args.device, cast_matrices=args.cast_matrices or bool(args.checkpoint),
+                 cache_dtype=args.cache_dtype)
     config_eos = getattr(model.config, "eos_token_id", None)
     if config_eos is not None:
         stop_ids.append(config_eos)
