@@ -116,35 +116,236 @@ __global__ void __launch_bounds__(128) write8_kernel(const GkPages8 p, const Wri
     if (lane == 0) (is_k ? p.k_exp : p.v_exp)[place] = (uint8_t)b;
 }
 
-// ------------------------------------------------------------------ read back
-// Block (page of the sequence, sequence): the page's keys and values of every kv head as bfloat16 under the same page number; zeros behind the
-// sequence's end.  Exact: e4m3 times a power of two.
-__global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int* __restrict__ kv_len, const int* __restrict__ slots, int last,
-                                                    __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out) {
+// The same for bfloat16 rows of 64 or 128: eight lanes a (token, head), which have HD / 16 neighbouring numbers of each half of the row in registers
+// from the load to the store.  Everything a lane needs is asked for at once.
+template <int E, typename T>
+__device__ __forceinline__ void load_run(const T* from, float (&v)[E]);
+template <>
+__device__ __forceinline__ void load_run<4, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[4]) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(from);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+template <>
+__device__ __forceinline__ void load_run<8, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(from);
+    const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(pairs[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void load_run<4, float>(const float* from, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(from);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+}
+template <>
+__device__ __forceinline__ void load_run<8, float>(const float* from, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(from + i);
+        v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+}
+
+template <int HD, typename TW>
+__global__ void __launch_bounds__(256) write8_wide_kernel(const GkPages8 p, const Write8 a) {
+    constexpr int E = HD / 16, HALF = HD / 2;
     pdl_launch_dependents();
     pdl_wait();
-    const int seq = blockIdx.y, index = blockIdx.x, d = p.head_dim;
-    const int len = length_of(p, kv_len[seq]);
-    if ((long long)index * p.page_size >= len) return;
-    if (last > 0 && (index + 1) * (long long)p.page_size <= (long long)len - last) return;
-    const int page = page_of(p, slots[seq], index);
-    if (page < 0) return;
-    const int rows = min(p.page_size, len - index * p.page_size), pairs = d >> 1;
-    const size_t base = (size_t)page * p.n_kv * p.page_size;
-    for (int i = threadIdx.x; i < p.n_kv * p.page_size * pairs; i += blockDim.x) {
-        const int place = i / pairs, c = (i - place * pairs) * 2, row = place % p.page_size;
-        __nv_bfloat162 k = __floats2bfloat162_rn(0.f, 0.f), v = k;
-        if (row < rows) {
-            const size_t at = (base + place) * d + c;
-            const float fk = power_of(p.k_exp[base + place]), fv = power_of(p.v_exp[base + place]);
-            const float2 x = floats2(*reinterpret_cast<const uint16_t*>(p.k + at)), y = floats2(*reinterpret_cast<const uint16_t*>(p.v + at));
-            k = __floats2bfloat162_rn(x.x * fk, x.y * fk);
-            v = __floats2bfloat162_rn(y.x * fv, y.y * fv);
+    const int n_heads = a.n_q + 2 * p.n_kv, sub = threadIdx.x & 7;
+    const long long item = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
+    const bool valid = item < (long long)a.n_tokens * n_heads;  // every lane stays for the shuffles
+    const int t = valid ? (int)(item / n_heads) : 0, head = valid ? (int)(item - (long long)t * n_heads) : 0;
+    const bool is_q = head < a.n_q, is_k = !is_q && head < a.n_q + p.n_kv;
+    const int pos = a.tok_pos[t];
+    long long place = -1;
+    if (valid && !is_q && a.write_kv) place = place_of(p, a, t, pos, head - a.n_q - (is_k ? 0 : p.n_kv));
+    const __nv_bfloat16* in = (const __nv_bfloat16*)a.qkv + ((size_t)t * n_heads + head) * HD + sub * E;
+    float x[E], y[E];
+    load_run<E>(in, x);
+    load_run<E>(in + HALF, y);
+    bool good = true;
+    const unsigned row_lanes = 0xffu << (threadIdx.x & 24);  // the lanes of this row go one way
+    if (is_q || is_k) {
+        if (a.use_norm) {
+            const TW* w = (const TW*)(is_q ? a.wq : a.wk) + sub * E;
+            float u[E], v[E], ss = 0.f;
+            load_run<E>(w, u);
+            load_run<E>(w + HALF, v);
+#pragma unroll
+            for (int i = 0; i < E; ++i) ss += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(row_lanes, ss, o);
+            const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                x[i] = (x[i] * inv) * u[i];
+                y[i] = (y[i] * inv) * v[i];
+            }
         }
-        const size_t to = (base + place) * d + c;
-        *reinterpret_cast<__nv_bfloat162*>(k_out + to) = k;
-        *reinterpret_cast<__nv_bfloat162*>(v_out + to) = v;
+        if (a.cos_table) {
+            good = (unsigned)pos < (unsigned)a.table_positions;
+            if (good) {
+                float c[E], sn[E];
+                load_run<E>(a.cos_table + (size_t)pos * HALF + sub * E, c);
+                load_run<E>(a.sin_table + (size_t)pos * HALF + sub * E, sn);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const float u = x[i], v = y[i];
+                    x[i] = u * c[i] - v * sn[i];
+                    y[i] = v * c[i] + u * sn[i];
+                }
+            } else if (valid && p.error) {
+                *p.error = ERR_PLACE;
+            }
+        }
     }
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!valid || !good) return;
+    if (is_q) {
+        __nv_bfloat16* out = (__nv_bfloat16*)a.q_out + ((size_t)t * a.n_q + head) * HD + sub * E;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t two[E / 2];
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                const __nv_bfloat162 pair = h ? __floats2bfloat162_rn(y[i], y[i + 1]) : __floats2bfloat162_rn(x[i], x[i + 1]);
+                two[i / 2] = *reinterpret_cast<const uint32_t*>(&pair);
+            }
+            if constexpr (E == 8) *reinterpret_cast<uint4*>(out + h * HALF) = make_uint4(two[0], two[1], two[E / 2 - 2], two[E / 2 - 1]);
+            else *reinterpret_cast<uint2*>(out + h * HALF) = make_uint2(two[0], two[1]);
+        }
+        return;
+    }
+    if (place < 0) return;
+    const int b = exponent_byte(top);
+    const float back = power_back(b);
+    uint8_t* to = (is_k ? p.k : p.v) + place * HD + sub * E;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t four[E / 4];
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+            four[i / 4] = h ? pack2(y[i] * back, y[i + 1] * back) | pack2(y[i + 2] * back, y[i + 3] * back) << 16
+                            : pack2(x[i] * back, x[i + 1] * back) | pack2(x[i + 2] * back, x[i + 3] * back) << 16;
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(to + h * HALF) = make_uint2(four[0], four[E / 4 - 1]);
+        else *reinterpret_cast<uint32_t*>(to + h * HALF) = four[0];
+    }
+    if (sub == 0) (is_k ? p.k_exp : p.v_exp)[place] = (uint8_t)b;
+}
+
+// ------------------------------------------------------------------ read back
+// For attention over what was read: pages renumbered under a table, lengths and slots of their own, so that no number that cannot be reaches it; and
+// a row of values that holds a NaN becomes zeros with a NaN key, which a token that does not see it cannot meet (0 * NaN).
+struct Clean8 {
+    int *table, *kv_len, *slots;  // [n_seqs][per], [n_seqs], [n_seqs]; null: read back under the pages' own numbers
+    int per, own_numbers;         // pages a sequence; whether a page keeps its number or is seq * per + index
+};
+
+// N numbers of a row as bfloat16: e4m3 times a power of two, exact.
+template <int N>
+__device__ __forceinline__ void widen(const uint32_t* four, float f, uint32_t* out) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+        const float2 a = floats2((uint16_t)four[i]), b = floats2((uint16_t)(four[i] >> 16));
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(a.x * f, a.y * f), hi = __floats2bfloat162_rn(b.x * f, b.y * f);
+        out[2 * i] = *reinterpret_cast<const uint32_t*>(&lo);
+        out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&hi);
+    }
+}
+
+// Block (page of the sequence, sequence, kv head): the page's keys and values of the head as bfloat16; zeros behind the sequence's end.  HD / 16
+// lanes a row, sixteen numbers each; HD = 0: any size, two numbers at a time.
+template <int HD, bool CLEAN>
+__global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int* __restrict__ kv_len, const int* __restrict__ slots, int last,
+                                                    __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, const Clean8 clean) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int seq = blockIdx.y, index = blockIdx.x, hk = blockIdx.z, d = HD ? HD : p.head_dim;
+    int len = length_of(p, kv_len[seq]);
+    if (CLEAN && len > (long long)clean.per * p.page_size) {
+        if (p.error) *p.error = ERR_PLACE;
+        len = clean.per * p.page_size;
+    }
+    const bool seen = (long long)index * p.page_size < len && (last <= 0 || (index + 1) * (long long)p.page_size > (long long)len - last);
+    const int page = seen ? page_of(p, slots[seq], index) : -1;
+    int to_page = page;
+    if (CLEAN) {
+        to_page = clean.own_numbers ? max(page, 0) : seq * clean.per + index;
+        if (hk == 0 && threadIdx.x == 0) {
+            clean.table[seq * clean.per + index] = to_page;
+            if (index == 0) {
+                clean.kv_len[seq] = len;
+                clean.slots[seq] = seq;
+            }
+        }
+        if (!seen || (clean.own_numbers && page < 0)) return;
+    } else if (page < 0) {
+        return;
+    }
+    const int rows = page < 0 ? 0 : min(p.page_size, len - index * p.page_size);
+    const size_t from = ((size_t)max(page, 0) * p.n_kv + hk) * p.page_size, to = ((size_t)to_page * p.n_kv + hk) * p.page_size;
+    if constexpr (HD > 0) {
+        constexpr int LANES = HD / 16;
+        const int c = threadIdx.x % LANES * 16;
+        for (int row = threadIdx.x / LANES; row < p.page_size; row += 256 / LANES) {
+            uint32_t k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (row < rows) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p.k + (from + row) * HD + c), y = *reinterpret_cast<const uint4*>(p.v + (from + row) * HD + c);
+                const uint32_t ks[4] = {x.x, x.y, x.z, x.w}, vs[4] = {y.x, y.y, y.z, y.w};
+                widen<16>(ks, power_of(p.k_exp[from + row]), k);
+                widen<16>(vs, power_of(p.v_exp[from + row]), v);
+                if (CLEAN) {
+                    bool nan = false;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) nan |= __vcmpeq4(vs[i] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;
+                    const unsigned mine = ((1u << LANES) - 1) << ((threadIdx.x & 31) / LANES * LANES);
+                    if (__ballot_sync(mine, nan) & mine) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = 0u, k[i] = 0x7fff7fffu;
+                    }
+                }
+            }
+            store32(k_out + (to + row) * HD + c, k);
+            store32(v_out + (to + row) * HD + c, v);
+        }
+    } else {
+        const int pairs = d >> 1;
+        for (int i = threadIdx.x; i < p.page_size * pairs; i += 256) {
+            const int row = i / pairs, c = (i - row * pairs) * 2;
+            __nv_bfloat162 k = __floats2bfloat162_rn(0.f, 0.f), v = k;
+            if (row < rows) {
+                const float fk = power_of(p.k_exp[from + row]), fv = power_of(p.v_exp[from + row]);
+                const float2 x = floats2(*reinterpret_cast<const uint16_t*>(p.k + (from + row) * d + c));
+                const float2 y = floats2(*reinterpret_cast<const uint16_t*>(p.v + (from + row) * d + c));
+                k = __floats2bfloat162_rn(x.x * fk, x.y * fk);
+                v = __floats2bfloat162_rn(y.x * fv, y.y * fv);
+            }
+            *reinterpret_cast<__nv_bfloat162*>(k_out + (to + row) * d + c) = k;
+            *reinterpret_cast<__nv_bfloat162*>(v_out + (to + row) * d + c) = v;
+        }
+    }
+}
+
+template <bool CLEAN>
+int launch_read8(const GkPages8& p, const int* kv_len, const int* slots, int n_seqs, int most, int last, void* k_out, void* v_out, const Clean8& clean,
+                 cudaStream_t stream) {
+    const dim3 grid(most, n_seqs, p.n_kv);
+    __nv_bfloat16 *k = (__nv_bfloat16*)k_out, *v = (__nv_bfloat16*)v_out;
+    const bool wide = (((uintptr_t)k_out | (uintptr_t)v_out) & 31) == 0;  // 32-byte stores
+    if (p.head_dim == 128 && wide) gk_launch(read8_kernel<128, CLEAN>, grid, dim3(256), 0, stream, p, kv_len, slots, last, k, v, clean);
+    else if (p.head_dim == 64 && wide) gk_launch(read8_kernel<64, CLEAN>, grid, dim3(256), 0, stream, p, kv_len, slots, last, k, v, clean);
+    else if constexpr (!CLEAN) gk_launch(read8_kernel<0, CLEAN>, grid, dim3(256), 0, stream, p, kv_len, slots, last, k, v, clean);
+    else return gk_fail(GK_BAD_ARGUMENT, "read8: head_dim %d is not 64 or 128, or memory begins between 32 bytes", p.head_dim);
+    GK_CHECK_LAUNCH("read8");
+    return GK_OK;
 }
 
 }  // namespace
@@ -167,6 +368,15 @@ GK_EXPORT int gk_write8(const GkPages8* pages, const void* qkv, int dtype, const
     const Write8 a = {qkv, wq, wk, cos_table, sin_table, tok_pos, tok_seq, slots, q_out, n_tokens, n_q, n_seqs, table_positions, use_norm, write_kv, eps};
     const long long items = (long long)n_tokens * (n_q + 2 * pages->n_kv), blocks = (items + 3) / 4;
     GK_REQUIRE(blocks < 2147483647LL, "write8: too many tokens");
+    if (dtype == GK_BF16 && (pages->head_dim == 64 || pages->head_dim == 128) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)wq | (uintptr_t)wk |
+                                                                                  (uintptr_t)cos_table | (uintptr_t)sin_table) & 15) == 0) {
+        GK_DISPATCH_DTYPE(weight_dtype, TW, {
+            if (pages->head_dim == 64) gk_launch(write8_wide_kernel<64, TW>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, *pages, a);
+            else gk_launch(write8_wide_kernel<128, TW>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, *pages, a);
+        })
+        GK_CHECK_LAUNCH("write8");
+        return GK_OK;
+    }
     GK_DISPATCH_DTYPE(dtype, T, {
         GK_DISPATCH_DTYPE(weight_dtype, TW, {
             gk_launch(write8_kernel<T, TW>, dim3((unsigned)blocks), dim3(128), 0, (cudaStream_t)stream, *pages, a);
@@ -186,8 +396,18 @@ GK_EXPORT int gk_read8(const GkPages8* pages, const int* kv_len, const int* slot
     GK_REQUIRE(kv_len && slots && k_out && v_out, "read8: an array is missing");
     int most = (int)(((long long)max_kv_len + pages->page_size - 1) / pages->page_size);
     if (most > pages->max_pages) most = pages->max_pages;
-    gk_launch(read8_kernel, dim3(most, n_seqs), dim3(256), 0, (cudaStream_t)stream, *pages, kv_len, slots, last, (__nv_bfloat16*)k_out,
-              (__nv_bfloat16*)v_out);
-    GK_CHECK_LAUNCH("read8");
-    return GK_OK;
+    return launch_read8<false>(*pages, kv_len, slots, n_seqs, most, last, k_out, v_out, Clean8{}, (cudaStream_t)stream);
+}
+
+// The same for attention over what is read: `per` pages a sequence under numbers seq * per + index (`own_numbers`: their own), and `table`
+// [n_seqs][per], `len_out` and `slots_out` [n_seqs] to go with them.  Heads of 64 or 128.
+GK_EXPORT int gk_clean8(const GkPages8* pages, const int* kv_len, const int* slots, int n_seqs, int per, int own_numbers, int last, void* k_out, void* v_out,
+                        int* table, int* len_out, int* slots_out, void* stream) {
+    const int status = cache8::check(pages, "clean8");
+    if (status != GK_OK) return status;
+    GK_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && per > 0 && last >= 0 && (long long)n_seqs * per < 2147483647LL, "clean8: bad sizes n_seqs=%d per=%d last=%d",
+               n_seqs, per, last);
+    if (n_seqs == 0) return GK_OK;
+    GK_REQUIRE(kv_len && slots && k_out && v_out && table && len_out && slots_out, "clean8: an array is missing");
+    return launch_read8<true>(*pages, kv_len, slots, n_seqs, per, last, k_out, v_out, Clean8{table, len_out, slots_out, per, own_numbers}, (cudaStream_t)stream);
 }

@@ -2579,17 +2579,97 @@ def _check_queries8(q: torch.Tensor, kv: PagedKV8, out: torch.Tensor | None) -> 
     return out
 
 
+ROWS8_HEAD_DIMS = (64, 128)
+ROWS8_MAX_GROUP = 16
+
+
+@functools.lru_cache(maxsize=None)
+def rows8_places(head_dim: int, rows: int, sm_count: int) -> tuple[int, int, int, int]:
+    """How many clusters of 1, 2, 4 and 8 blocks of the kernel for few rows over 8-bit pages the device holds at once.  Asked of the device where there
+    is one; three blocks an SM (two of sixteen rows) otherwise."""
+    if torch.cuda.is_available():
+        from .library import library
+
+        got = tuple(library().gk_rows8_places(int(head_dim), int(rows), c) for c in (1, 2, 4, 8))
+        if all(g > 0 for g in got):
+            return got
+    return tuple((3 if rows == 8 else 2) * sm_count // c for c in (1, 2, 4, 8))
+
+
+@functools.lru_cache(maxsize=4096)
+def rows8_cut(pairs: int, kv_len: int, places: tuple[int, int, int, int]) -> tuple[int, int]:
+    """How the keys of ``pairs`` (row tile, kv head) pairs are shared out: (1, 2, 4 or 8, 0): so many blocks, a cluster, a pair; (0, n): all pairs' keys in
+    about ``n`` pieces of one size and at most one more a pair, joined by a second kernel.
+
+    The lowest estimate, in steps of 32 keys of a warp (0.75 us where a warp has a scheduler to itself): waves of clusters x (steps of a warp + 5
+    for what a block does besides), or steps + 5 + 4 for pieces and the second kernel, which are only taken where they are one wave and half the places
+    are left for them.  Measured, us with 1, 2, 4, 8 blocks a pair and with 296 pieces, 16/8 heads of 128, sequences of one length: 1 of 16,000 tokens
+    98 / 52 / 30 / 17.3 / 15.4; 4 of 4,000 28.5 / 17.2 / 11.3 / 10.1 / 13.4; 8 of 1,000 10.3 / 8.1 / 7.7 / 12.3 / 10.8; 16 of 2,000
+    19.5 / 16.4 / 23.5 / 26.6 / 19.1; 32 of 4,000 45 / 63 / 56 / 68 / 65; 64 of 4,000 111 / 97 / 95 / 120 / 115."""
+    tiles = max(1, -(-kv_len // 32))
+
+    def estimate(index: int) -> float:
+        splits = 1 << index
+        return -(-pairs // places[index]) * (-(-tiles // (4 * splits)) + 5)
+
+    best = min((i for i in range(4) if i == 0 or tiles >= 2 << i), key=estimate)
+    pieces = places[0] - pairs
+    if pieces >= places[0] // 2 and pairs * tiles / (4 * pieces) + 9 < estimate(best):
+        return 0, pieces
+    return 1 << best, 0
+
+
+def _rows8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor | None, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, kv_len_hint: int,
+           scale: float, window: int, sink: bool, cut: tuple[int, int] | None, out: torch.Tensor) -> torch.Tensor:
+    n_seqs, n_q, d = kv_len.shape[0], q.shape[1], q.shape[2]
+    n_kv = kv.k.shape[1]
+    n_rows = max_q_len * (n_q // n_kv)
+    rows = 8 if n_rows <= 8 else 16
+    pairs = n_seqs * -(-n_rows // rows) * n_kv
+    if cut is None:
+        cut = rows8_cut(pairs, min(kv_len_hint, window + max_q_len) if window else kv_len_hint, rows8_places(d, rows, sm_count(q.device)))
+    splits, pieces = cut
+    scratch = None
+    if splits == 0:
+        scratch = torch.empty(((pieces + pairs) * rows * (d + 3),), dtype=torch.float32, device=q.device)
+    call("gk_rows8", kv._at, ptr(q), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), n_seqs, n_q, max_q_len, rows, splits, pieces, ptr(scratch),
+         float(scale), int(window), int(sink), stream_ptr())
+    return out
+
+
 def attention_decode8(q: torch.Tensor, kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, scale: float, window: int = 0,
-                      sink: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+                      sink: bool = False, out: torch.Tensor | None = None, cut: tuple[int, int] | None = None) -> torch.Tensor:
     """Attention of one new token per sequence (``q [n_seqs, n_q, d]``, bfloat16 or float32) over 8-bit pages; ``kv_len[i]`` counts the sequence's
-    cached tokens including the new one, ``max_kv_len`` is the longest of them or a bound on it.  ``sink``: one more term in the softmax's
-    denominator, a key of score 0 without a value.  A sequence without tokens gets zeros."""
+    cached tokens including the new one; ``max_kv_len``, about the longest of them, is what the launch's shape goes by.  ``sink``: one more term in
+    the softmax's denominator, a key of score 0 without a value.  ``cut``: how the keys are shared out (``rows8_cut``; None: chosen
+    here).  A sequence without tokens gets zeros."""
     out = _check_queries8(q, kv, out)
     n, n_q, d = q.shape
     _check8(kv, q, ("kv_len", kv_len, n), ("slots", slots, n))
+    if q.dtype == torch.bfloat16 and d in ROWS8_HEAD_DIMS and kv.k.shape[2] == 64 and n_q // kv.k.shape[1] <= ROWS8_MAX_GROUP:
+        return _rows8(q, kv, None, kv_len, slots, 1, max_kv_len, scale, window, sink, cut, out)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), None, ptr(kv_len), ptr(slots), n, n, n_q, float(scale), int(window), int(sink),
          stream_ptr())
     return out
+
+
+# Rows (tokens x query heads of a kv head) of a sequence up to which several tokens go through the kernel for few rows.
+ROWS8_PROMPT_MAX = 64
+
+
+def _clean_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, last: int) -> tuple[PagedKV, torch.Tensor, torch.Tensor]:
+    """The step's pages as bfloat16 with a table, lengths and slots of their own.  Where the sequences could have more pages than there are, pages keep
+    their numbers."""
+    n, device = kv_len.shape[0], kv.k.device
+    per = min(max(1, -(-int(max_kv_len) // kv.page_size)), kv.max_pages)
+    own_numbers = n * per > kv.k.shape[0]
+    shape = (kv.k.shape[0] if own_numbers else n * per, *kv.k.shape[1:])
+    k, v = (torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(2))
+    ints = torch.empty((n * per + 2 * n,), dtype=torch.int32, device=device)
+    table, lens, own_slots = ints[: n * per].view(n, per), ints[n * per: n * per + n], ints[n * per + n:]
+    call("gk_clean8", kv._at, ptr(kv_len), ptr(slots), n, per, int(own_numbers), int(last), ptr(k), ptr(v), ptr(table), ptr(lens), ptr(own_slots),
+         stream_ptr())
+    return PagedKV(k, v, table), lens, own_slots
 
 
 def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, max_kv_len: int,
@@ -2600,6 +2680,12 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     out = _check_queries8(q, kv, out)
     n_seqs = kv_len.shape[0]
     _check8(kv, q, ("cu_q", cu_q, n_seqs + 1), ("kv_len", kv_len, n_seqs), ("slots", slots, n_seqs))
+    group = q.shape[1] // kv.k.shape[1]
+    if q.dtype == torch.bfloat16 and q.shape[2] in ROWS8_HEAD_DIMS and kv.k.shape[2] == 64 and group <= ROWS8_MAX_GROUP and n_seqs and q.shape[0]:
+        if max_q_len * group <= ROWS8_PROMPT_MAX:
+            return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
+        pages, lens, own_slots = _clean_pages8(kv, kv_len, slots, max_kv_len, window + max_q_len if window else 0)
+        return attention_prefill(q, pages, cu_q, lens, own_slots, max_q_len, scale, window, out, sink=sink)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
          int(window), int(sink), stream_ptr())
     return out

@@ -210,14 +210,15 @@ def sequences(lens, n_kv, d, page=PAGE, key_scale=1.0, window=0, new=None):
 GROUPS = [(1, 1, 128), (4, 2, 128), (16, 4, 128), (8, 1, 128), (12, 1, 128), (16, 1, 64), (6, 2, 64), (17, 1, 64), (6, 2, 80), (3, 3, 16)]
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dtype,cut", [(torch.bfloat16, None), (torch.bfloat16, (1, 0)), (torch.bfloat16, (3, 0)), (torch.bfloat16, (8, 0)),
+                                       (torch.bfloat16, (0, 1)), (torch.bfloat16, (0, 40)), (torch.float32, None)])
 @pytest.mark.parametrize("n_q,n_kv,d", GROUPS)
 @pytest.mark.parametrize("window,sink", [(0, False), (70, True)])
-def test_decode(dtype, n_q, n_kv, d, window, sink):
+def test_decode(dtype, cut, n_q, n_kv, d, window, sink):
     lens = [1, 64, 65, 300, 777, 0, 16]
     kv, slots, table = sequences(lens, n_kv, d, window=window)
     q = rand(len(lens), n_q, d, seed=5).to(dtype)
-    got = F().attention_decode8(q.to(DEV), kv, ints(*lens), slots, 777, d**-0.5, window, sink)
+    got = F().attention_decode8(q.to(DEV), kv, ints(*lens), slots, 777, d**-0.5, window, sink, cut=cut)
     assert (got[5] == 0).all()  # a sequence without tokens
     for i, n in enumerate(lens):
         if n:
@@ -285,6 +286,39 @@ def test_numbers_that_are_none(n_q, n_kv, d):
     assert torch.isfinite(inside).all()
 
 
+@pytest.mark.parametrize("n_q,n_kv,d", [(4, 2, 128), (6, 2, 64), (6, 2, 80)])
+@pytest.mark.parametrize("m", [5, 90])
+@pytest.mark.parametrize("window", [0, 40])
+def test_values_that_are_none_reach_only_who_sees_them(n_q, n_kv, d, m, window):
+    """A value that holds a NaN: tokens in front of it, tokens whose window has left it and other heads do not meet it."""
+    n, group = 150, n_q // n_kv
+    kv, slots, table = sequences([n, 80], n_kv, d)
+    at = n - m + 2  # the step's third token
+    for name in ("k", "v"):
+        kv_bytes = getattr(kv, name).view(torch.uint8)
+        if name == "v":
+            kv_bytes[int(table[int(slots[0]), at // PAGE]), 1, at % PAGE, 7] = 0xFF
+    q = rand(m + 3, n_q, d, seed=5).to(torch.bfloat16).to(DEV)
+    got = F().attention_prefill8(q, kv, ints(0, m, m + 3), ints(n, 80), slots, m, n, d**-0.5, window)
+    see = torch.tensor([t >= 2 and (not window or n - m + t < at + window) for t in range(m)])
+    assert torch.isfinite(got[m:]).all() and torch.isfinite(got[:m, :group]).all()
+    assert torch.isfinite(got[:m, group:2 * group][~see]).all()
+    assert torch.isnan(got[:m, group:2 * group][see][:, :, 7]).all()
+
+
+def test_prefill_where_pages_keep_their_numbers():
+    """Bounds on lengths so large that renumbered pages would be more than there are."""
+    n_q, n_kv, d, new, lens = 4, 2, 128, [70, 1, 40], [200, 64, 40]
+    kv, slots, table = sequences(lens, n_kv, d, new=new)
+    wide = torch.cat([kv.block_table, torch.zeros((kv.block_table.shape[0], 60), dtype=torch.int32, device=DEV)], 1).contiguous()
+    wide = F().PagedKV8(kv.k, kv.v, kv.k_exp, kv.v_exp, wide)
+    q = rand(111, n_q, d, seed=5).to(torch.bfloat16)
+    args = (ints(0, 70, 71, 111), ints(*lens), slots, 70)
+    got = F().attention_prefill8(q.to(DEV), wide, *args, 64 * 60, d**-0.5)
+    assert torch.equal(got, F().attention_prefill8(q.to(DEV), kv, *args, 200, d**-0.5))
+    F().check_kernel_errors(DEV)
+
+
 def test_page_numbers_slots_and_lengths_that_cannot_be():
     """They are skipped and reported; the step's other sequences are what they are."""
     n_q, n_kv, d = 4, 2, 128
@@ -294,6 +328,9 @@ def test_page_numbers_slots_and_lengths_that_cannot_be():
     args = (kv, ints(*lens), slots, 100, d**-0.5)
     good = F().attention_decode8(q, *args)
     F().check_kernel_errors(DEV)
+    several = rand(120, n_q, d, seed=6).to(torch.bfloat16).to(DEV)
+    prompts = [(m, ints(0, m, 2 * m, 3 * m), F().attention_prefill8(several[: 3 * m], kv, ints(0, m, 2 * m, 3 * m), ints(*lens), slots, m, 100, d**-0.5))
+               for m in (3, 40)]  # through both kernels
     keep = kv.block_table.clone()
     for wrong in (-1, kv.k.shape[0], 2**31 - 1):
         kv.block_table[int(slots[1]), 1] = wrong
@@ -301,6 +338,11 @@ def test_page_numbers_slots_and_lengths_that_cannot_be():
         with pytest.raises(Exception, match="page number"):
             F().check_kernel_errors(DEV)
         assert torch.equal(got[[0, 2]], good[[0, 2]])
+        for m, cu, want in prompts:
+            got = F().attention_prefill8(several[: 3 * m], kv, cu, ints(*lens), slots, m, 100, d**-0.5)
+            with pytest.raises(Exception, match="page number"):
+                F().check_kernel_errors(DEV)
+            assert torch.equal(got[:m], want[:m]) and torch.equal(got[2 * m:], want[2 * m:])
         F().read_pages8(kv, ints(*lens), slots, 100)
         with pytest.raises(Exception, match="page number"):
             F().check_kernel_errors(DEV)
