@@ -23,6 +23,8 @@
 // library's split leaves 23 KB an SM); scores by products of e4m3 numbers with the query as the sum of two of them (117 against 116: sm_100a makes
 // halves of them under the hood); the scores of the next keys under the exponentials of these (116, no gain).
 
+#include <atomic>
+
 #include "cache8.cuh"
 
 namespace {
@@ -642,7 +644,13 @@ int places_of(int cluster) {
 template <int D, int NT>
 int launch_rows8(const GkPages8& p, const Rows8& a, cudaStream_t stream) {
     const int smem = (int)sizeof(Smem8<D, NT>);
-    cudaError_t err = cudaFuncSetAttribute(rows8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<unsigned long long> configured{0};  // a bit a device (the attribute is the device's)
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err == cudaSuccess && (device > 63 || !(configured.load() >> device & 1))) {
+        err = cudaFuncSetAttribute(rows8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (err == cudaSuccess && device <= 63) configured.fetch_or(1ull << device);
+    }
     if (err != cudaSuccess) return gk_fail(GK_CUDA_ERROR, "rows8: %s", cudaGetErrorString(err));
     if (a.n_splits > 0) {
         gk_launch_cluster(rows8_kernel<D, NT>, dim3(a.n_splits, p.n_kv, a.n_units), dim3(THREADS), smem, stream, dim3(a.n_splits, 1, 1), p, a);

@@ -1,8 +1,11 @@
 // Writing keys and values into the 8-bit cache, and reading them back (what is kept: cache8.cuh).
 //
 // The write does the attention input stage too, as the 16-bit cache's does: per-head RMSNorm of q and k (src/layers/rmsnorm.py:11-16),
-// rotation (src/layers/rope.py:17-33), order of src/layers/attention.py:82-89.  All of it is 32-bit up to the one rounding of
-// each result: q to its type, k and v to e4m3.
+// rotation (src/layers/rope.py:17-33), order of src/layers/attention.py:82-89.  Queries are 32-bit up to the one rounding to their type, values are only
+// rounded.  Keys come out as the formula in 64 bits rounded once: e4m3's steps are so coarse that a number 2^-22 beside the middle between two of
+// them goes wrong by a sixteenth of itself, which 32 bits do to some three in a million.  All of it in 64 bits is slow (7,921 tokens of 32/8 heads of
+// 128: 50 us more), so the wide kernel makes them in 32 bits and does over, in 64, the rows that have a number or their maximum next to a border:
+// one in some fifty.
 
 #include "cache8.cuh"
 
@@ -20,15 +23,71 @@ struct Write8 {
     float eps;
 };
 
-// The byte that a k or v row's place begins at, or null.
-__device__ __forceinline__ long long place_of(const GkPages8& p, const Write8& a, int t, int pos, int hk) {
-    const int seq = a.tok_seq[t];
+// A 64-bit number as 32 bits to be rounded on: what is cut off leaves its mark in the last bit, so that the second rounding is that of the number itself.
+__device__ __forceinline__ float to_be_rounded(double x) {
+    const float f = __double2float_rz(x);
+    return (double)f == x || f != f ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// RMSNorm and rotation of a row whose lanes hold N pairs each, pair i of a lane at `at(i)` of the halves; `lanes`: the row's, a power of two of them.
+// Returns whether the position is one of the rotation's.
+template <typename R, int N, typename TW, typename At>
+__device__ __forceinline__ bool norm_rotate(R (&x)[N], R (&y)[N], const Write8& a, const TW* w, int half, int pos, int lanes, unsigned mask, At at) {
+    if (a.use_norm) {
+        R ss = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss += x[i] * x[i] + y[i] * y[i];
+        for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const R inv = (R)1 / sqrt(ss / (R)(2 * half) + (R)a.eps);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at(i) < half) {
+                x[i] = (x[i] * inv) * (R)to_float(w[at(i)]);
+                y[i] = (y[i] * inv) * (R)to_float(w[at(i) + half]);
+            }
+    }
+    if (a.cos_table) {
+        if ((unsigned)pos >= (unsigned)a.table_positions) return false;
+        const float *cs = a.cos_table + (size_t)pos * half, *sn = a.sin_table + (size_t)pos * half;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at(i) < half) {
+                const R c = cs[at(i)], s = sn[at(i)], u = x[i], v = y[i];
+                x[i] = u * c - v * s;
+                y[i] = v * c + u * s;
+            }
+    }
+    return true;
+}
+
+// A row's numbers as bytes and the byte of its power; pair i of a lane at `at(i)` of the halves.
+template <int N, typename At>
+__device__ __forceinline__ void store_bytes(const float (&x)[N], const float (&y)[N], uint8_t* to, uint8_t* to_exp, int half, int lanes, unsigned mask, bool first,
+                                            At at) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
+    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+    const int b = exponent_byte(top);
+    const float back = power_back(b);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (at(i) < half) {
+            const uint32_t two = pack2(x[i] * back, y[i] * back);
+            to[at(i)] = (uint8_t)two;
+            to[at(i) + half] = (uint8_t)(two >> 8);
+        }
+    if (first) *to_exp = (uint8_t)b;
+}
+
+// The place of a token's row of kv head 0, counted in rows (the next head's is a page further), or -1.
+__device__ __forceinline__ long long place_of(const GkPages8& p, const Write8& a, int seq, int pos) {
     if ((unsigned)seq >= (unsigned)a.n_seqs || pos < 0) {
         if (p.error) *p.error = ERR_PLACE;
         return -1;
     }
     const int page = page_of(p, a.slots[seq], pos / p.page_size);
-    return page < 0 ? -1 : ((long long)page * p.n_kv + hk) * p.page_size + pos % p.page_size;
+    return page < 0 ? -1 : (long long)page * p.n_kv * p.page_size + pos % p.page_size;
 }
 
 // A warp a (token, head): lane l has the pairs (i, i + head_dim / 2) of the rotation for i = l, l + 32, ...
@@ -52,72 +111,41 @@ __global__ void __launch_bounds__(128) write8_kernel(const GkPages8 p, const Wri
         x[i] = c < half ? to_float(in[c]) : 0.f;
         y[i] = c < half ? to_float(in[c + half]) : 0.f;
     }
-    if (is_q || is_k) {
-        if (a.use_norm) {
-            const TW* w = (const TW*)(is_q ? a.wq : a.wk);
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < MAXP; ++i) ss += x[i] * x[i] + y[i] * y[i];
-            const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)d + a.eps);
-#pragma unroll
-            for (int i = 0; i < MAXP; ++i) {
-                const int c = lane + 32 * i;
-                if (c < half) {
-                    x[i] = (x[i] * inv) * to_float(w[c]);
-                    y[i] = (y[i] * inv) * to_float(w[c + half]);
-                }
-            }
-        }
-        if (a.cos_table) {
-            if ((unsigned)pos >= (unsigned)a.table_positions) {
-                if (p.error && lane == 0) *p.error = ERR_PLACE;
-                return;
-            }
-#pragma unroll
-            for (int i = 0; i < MAXP; ++i) {
-                const int c = lane + 32 * i;
-                if (c < half) {
-                    const float cs = a.cos_table[(size_t)pos * half + c], sn = a.sin_table[(size_t)pos * half + c], u = x[i], v = y[i];
-                    x[i] = u * cs - v * sn;
-                    y[i] = v * cs + u * sn;
-                }
-            }
-        }
-    }
+    const auto at = [&](int i) { return lane + 32 * i; };
     if (is_q) {
+        if (!norm_rotate(x, y, a, (const TW*)a.wq, half, pos, 32, 0xffffffffu, at)) {
+            if (p.error && lane == 0) *p.error = ERR_PLACE;
+            return;
+        }
         T* out = (T*)a.q_out + ((size_t)t * a.n_q + head) * d;
 #pragma unroll
-        for (int i = 0; i < MAXP; ++i) {
-            const int c = lane + 32 * i;
-            if (c < half) {
-                out[c] = from_float<T>(x[i]);
-                out[c + half] = from_float<T>(y[i]);
+        for (int i = 0; i < MAXP; ++i)
+            if (at(i) < half) {
+                out[at(i)] = from_float<T>(x[i]);
+                out[at(i) + half] = from_float<T>(y[i]);
             }
-        }
         return;
     }
-    const long long place = place_of(p, a, t, pos, head - a.n_q - (is_k ? 0 : p.n_kv));
-    if (place < 0) return;
-    float top = 0.f;
+    long long place = place_of(p, a, a.tok_seq[t], pos);
+    if (place >= 0) place += (long long)(head - a.n_q - (is_k ? 0 : p.n_kv)) * p.page_size;
+    if (is_k) {
+        double u[MAXP], v[MAXP];
 #pragma unroll
-    for (int i = 0; i < MAXP; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
-    const int b = exponent_byte(warp_max(top));
-    const float back = power_back(b);
-    uint8_t* to = (is_k ? p.k : p.v) + place * d;
-#pragma unroll
-    for (int i = 0; i < MAXP; ++i) {
-        const int c = lane + 32 * i;
-        if (c < half) {
-            const uint32_t two = pack2(x[i] * back, y[i] * back);
-            to[c] = (uint8_t)two;
-            to[c + half] = (uint8_t)(two >> 8);
+        for (int i = 0; i < MAXP; ++i) u[i] = x[i], v[i] = y[i];
+        if (!norm_rotate(u, v, a, (const TW*)a.wk, half, pos, 32, 0xffffffffu, at)) {
+            if (p.error && lane == 0) *p.error = ERR_PLACE;
+            return;
         }
+#pragma unroll
+        for (int i = 0; i < MAXP; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
     }
-    if (lane == 0) (is_k ? p.k_exp : p.v_exp)[place] = (uint8_t)b;
+    if (place >= 0) store_bytes(x, y, (is_k ? p.k : p.v) + place * d, (is_k ? p.k_exp : p.v_exp) + place, half, 32, 0xffffffffu, lane == 0, at);
 }
 
-// The same for bfloat16 rows of 64 or 128: eight lanes a (token, head), which have HD / 16 neighbouring numbers of each half of the row in registers
-// from the load to the store.  Everything a lane needs is asked for at once.
+// bfloat16 rows of 64 or 128: eight lanes a row, which have HD / 16 neighbouring numbers of each half of it.  A task is 4 R rows of one token (its
+// queries first, then keys and values), a warp's.  Few tokens: four rows, everything asked for at once (`write8_wide_kernel`).  Many: sixteen, by
+// warps that stay and have the next task's rows and rotation under way in shared memory while they make this one's (`write8_stream_kernel`).  Bound by
+// memory then; through registers the same work is bound by what may be under way in L1, of which the library's shared-memory split leaves 23 KB an SM.
 template <int E, typename T>
 __device__ __forceinline__ void load_run(const T* from, float (&v)[E]);
 template <>
@@ -150,67 +178,69 @@ __device__ __forceinline__ void load_run<8, float>(const float* from, float (&v)
     }
 }
 
+// A key in 64 bits, by the eight lanes of its row.
 template <int HD, typename TW>
-__global__ void __launch_bounds__(256) write8_wide_kernel(const GkPages8 p, const Write8 a) {
+__device__ __noinline__ void write_key_64(const GkPages8& p, const Write8& a, const __nv_bfloat16* row, int pos, long long place, int sub, unsigned mask) {
     constexpr int E = HD / 16, HALF = HD / 2;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int n_heads = a.n_q + 2 * p.n_kv, sub = threadIdx.x & 7;
-    const long long item = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
-    const bool valid = item < (long long)a.n_tokens * n_heads;  // every lane stays for the shuffles
-    const int t = valid ? (int)(item / n_heads) : 0, head = valid ? (int)(item - (long long)t * n_heads) : 0;
-    const bool is_q = head < a.n_q, is_k = !is_q && head < a.n_q + p.n_kv;
-    const int pos = a.tok_pos[t];
-    long long place = -1;
-    if (valid && !is_q && a.write_kv) place = place_of(p, a, t, pos, head - a.n_q - (is_k ? 0 : p.n_kv));
-    const __nv_bfloat16* in = (const __nv_bfloat16*)a.qkv + ((size_t)t * n_heads + head) * HD + sub * E;
+    const auto at = [&](int i) { return sub * E + i; };
     float x[E], y[E];
-    load_run<E>(in, x);
-    load_run<E>(in + HALF, y);
-    bool good = true;
-    const unsigned row_lanes = 0xffu << (threadIdx.x & 24);  // the lanes of this row go one way
-    if (is_q || is_k) {
+    double u[E], v[E];
+    load_run<E>(row + sub * E, x);
+    load_run<E>(row + HALF + sub * E, y);
+#pragma unroll
+    for (int i = 0; i < E; ++i) u[i] = x[i], v[i] = y[i];
+    norm_rotate(u, v, a, (const TW*)a.wk, HALF, pos, 8, mask, at);
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
+    store_bytes(x, y, p.k + place * HD, p.k_exp + place, HALF, 8, mask, sub == 0, at);
+}
+
+// Whether `y`, scaled and rounded to `got`, lies within `tol` of the middle between two e4m3 numbers.
+__device__ __forceinline__ bool near_middle(float y, float got, float tol) {
+    const uint32_t power = max(__float_as_uint(fabsf(y)) & 0x7f800000u, 0x3c800000u);  // 2^-6 at the least
+    return __uint_as_float(power - (4u << 23)) - fabsf(y - got) < tol;
+}
+
+template <int E>
+__device__ __forceinline__ float sum_of_squares(const float (&x)[E], const float (&y)[E]) {  // a tree: seven roundings in a row with the lanes' three
+    float s[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[i] = fmaf(x[i], x[i], y[i] * y[i]);
+#pragma unroll
+    for (int n = E / 2; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) s[i] += s[i + n];
+    return s[0];
+}
+
+// A row in a lane group's registers to where it belongs: a query (place < 0), a key or a value.
+template <int HD, typename TW>
+__device__ __forceinline__ void finish_row(const GkPages8& p, const Write8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16],
+                                           const float (&w1)[HD / 16], const float (&c)[HD / 16], const float (&sn)[HD / 16], bool turns, bool is_v,
+                                           __nv_bfloat16* q_out, const __nv_bfloat16* in, int pos, long long place, int sub, unsigned mask) {
+    constexpr int E = HD / 16, HALF = HD / 2;
+    if (!is_v) {
         if (a.use_norm) {
-            const TW* w = (const TW*)(is_q ? a.wq : a.wk) + sub * E;
-            float u[E], v[E], ss = 0.f;
-            load_run<E>(w, u);
-            load_run<E>(w + HALF, v);
+            float ss = sum_of_squares(x, y);
 #pragma unroll
-            for (int i = 0; i < E; ++i) ss += x[i] * x[i] + y[i] * y[i];
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(row_lanes, ss, o);
-            const float inv = 1.0f / sqrtf(ss / (float)HD + a.eps);
+            for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+            const float inv = rsqrtf(fmaf(ss, 1.f / HD, a.eps));
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                x[i] = (x[i] * inv) * u[i];
-                y[i] = (y[i] * inv) * v[i];
+                x[i] = (x[i] * inv) * w0[i];
+                y[i] = (y[i] * inv) * w1[i];
             }
         }
-        if (a.cos_table) {
-            good = (unsigned)pos < (unsigned)a.table_positions;
-            if (good) {
-                float c[E], sn[E];
-                load_run<E>(a.cos_table + (size_t)pos * HALF + sub * E, c);
-                load_run<E>(a.sin_table + (size_t)pos * HALF + sub * E, sn);
+        if (turns) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const float u = x[i], v = y[i];
-                    x[i] = u * c[i] - v * sn[i];
-                    y[i] = v * c[i] + u * sn[i];
-                }
-            } else if (valid && p.error) {
-                *p.error = ERR_PLACE;
+            for (int i = 0; i < E; ++i) {
+                const float u = x[i], v = y[i];
+                x[i] = u * c[i] - v * sn[i];
+                y[i] = v * c[i] + u * sn[i];
             }
         }
     }
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!valid || !good) return;
-    if (is_q) {
-        __nv_bfloat16* out = (__nv_bfloat16*)a.q_out + ((size_t)t * a.n_q + head) * HD + sub * E;
+    if (q_out) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint32_t two[E / 2];
@@ -219,26 +249,229 @@ __global__ void __launch_bounds__(256) write8_wide_kernel(const GkPages8 p, cons
                 const __nv_bfloat162 pair = h ? __floats2bfloat162_rn(y[i], y[i + 1]) : __floats2bfloat162_rn(x[i], x[i + 1]);
                 two[i / 2] = *reinterpret_cast<const uint32_t*>(&pair);
             }
-            if constexpr (E == 8) *reinterpret_cast<uint4*>(out + h * HALF) = make_uint4(two[0], two[1], two[E / 2 - 2], two[E / 2 - 1]);
-            else *reinterpret_cast<uint2*>(out + h * HALF) = make_uint2(two[0], two[1]);
+            if constexpr (E == 8) *reinterpret_cast<uint4*>(q_out + sub * E + h * HALF) = make_uint4(two[0], two[1], two[E / 2 - 2], two[E / 2 - 1]);
+            else *reinterpret_cast<uint2*>(q_out + sub * E + h * HALF) = make_uint2(two[0], two[1]);
         }
         return;
     }
-    if (place < 0) return;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
     const int b = exponent_byte(top);
     const float back = power_back(b);
-    uint8_t* to = (is_k ? p.k : p.v) + place * HD + sub * E;
+    uint32_t four[2][E / 4];
+    bool unsure = abs((int)(__float_as_uint(top) & 0x7fffffu) - 0x600000) < 32;  // 2^-18 of the border between two powers
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+            const float u[4] = {(h ? y : x)[i] * back, (h ? y : x)[i + 1] * back, (h ? y : x)[i + 2] * back, (h ? y : x)[i + 3] * back};
+            const uint32_t lo = pack2(u[0], u[1]), hi = pack2(u[2], u[3]);
+            four[h][i / 4] = lo | hi << 16;
+            if (!is_v) {
+                const float2 g0 = floats2((uint16_t)lo), g1 = floats2((uint16_t)hi);
+                const float got[4] = {g0.x, g0.y, g1.x, g1.y};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // 1.5 * 2^-21 of the number for the norm's factor, 2^-22 of both numbers that the rotation mixes for the roundings of its
+                    // products, twice
+                    const float other = fabsf((h ? x : y)[i + e] * back);
+                    unsure |= near_middle(u[e], got[e], fmaf(4.76837158e-7f, other, 1.19209290e-6f * fabsf(u[e])));
+                }
+            }
+        }
+    if (!is_v && (a.use_norm || turns) && __any_sync(mask, unsure)) {
+        write_key_64<HD, TW>(p, a, in, pos, place, sub, mask);
+        return;
+    }
+    uint8_t* to = (is_v ? p.v : p.k) + place * HD + sub * E;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint32_t four[E / 4];
-#pragma unroll
-        for (int i = 0; i < E; i += 4)
-            four[i / 4] = h ? pack2(y[i] * back, y[i + 1] * back) | pack2(y[i + 2] * back, y[i + 3] * back) << 16
-                            : pack2(x[i] * back, x[i + 1] * back) | pack2(x[i + 2] * back, x[i + 3] * back) << 16;
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(to + h * HALF) = make_uint2(four[0], four[E / 4 - 1]);
-        else *reinterpret_cast<uint32_t*>(to + h * HALF) = four[0];
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(to + h * HALF) = make_uint2(four[h][0], four[h][E / 4 - 1]);
+        else *reinterpret_cast<uint32_t*>(to + h * HALF) = four[h][0];
     }
-    if (sub == 0) (is_k ? p.k_exp : p.v_exp)[place] = (uint8_t)b;
+    if (sub == 0) (is_v ? p.v_exp : p.k_exp)[place] = (uint8_t)b;
+}
+
+// A task: which token, which rows of it.
+struct Task8 {
+    int t, first, n_rows;  // rows first, first + 4, ... below n_rows of the queries, or of the keys and values
+    bool queries;
+    const __nv_bfloat16* in;
+};
+template <int HD, int R>
+__device__ __forceinline__ Task8 task_of(const GkPages8& p, const Write8& a, unsigned task, int q_tasks, int tasks, int lane_row) {
+    Task8 k;
+    // keys and values of all tokens first, then queries: a warp that stays has one kind of row, and its weights, for long
+    const unsigned kv_tasks = (unsigned)(tasks - q_tasks), kv_all = kv_tasks * (unsigned)a.n_tokens;
+    k.queries = task >= kv_all;
+    const unsigned of = k.queries ? task - kv_all : task, each = k.queries ? (unsigned)q_tasks : kv_tasks;
+    k.t = (int)(of / each);
+    k.first = (int)(of - (unsigned)k.t * each) * 4 * R + lane_row;
+    k.n_rows = k.queries ? a.n_q : 2 * p.n_kv;
+    k.in = (const __nv_bfloat16*)a.qkv + ((size_t)k.t * (a.n_q + 2 * p.n_kv) + (k.queries ? 0 : a.n_q)) * HD;
+    return k;
+}
+
+template <int HD, typename TW>
+__global__ void __launch_bounds__(128) write8_wide_kernel(const GkPages8 p, const Write8 a, int q_tasks, int tasks, unsigned n_tasks) {
+    constexpr int E = HD / 16, HALF = HD / 2;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int sub = threadIdx.x & 7;
+    const unsigned mask = 0xffu << (threadIdx.x & 24), task = blockIdx.x * 4 + (threadIdx.x >> 5);  // the lanes of a row go one way
+    if (task >= n_tasks) return;
+    const Task8 k = task_of<HD, 1>(p, a, task, q_tasks, tasks, (threadIdx.x & 31) >> 3);
+    if (k.first >= k.n_rows) return;
+    const int pos = a.tok_pos[k.t];
+    const __nv_bfloat16* in = k.in + (size_t)k.first * HD;
+    float x[E], y[E], w0[E], w1[E], c[E], sn[E];
+    load_run<E>(in + sub * E, x);
+    load_run<E>(in + HALF + sub * E, y);
+    if (a.use_norm) {
+        const TW* w = (const TW*)(k.queries ? a.wq : a.wk) + sub * E;
+        load_run<E>(w, w0);
+        load_run<E>(w + HALF, w1);
+    }
+    const bool is_v = !k.queries && k.first >= p.n_kv, turns = a.cos_table != nullptr && !is_v;
+    if (turns) {
+        if ((unsigned)pos >= (unsigned)a.table_positions) {
+            if (p.error) *p.error = ERR_PLACE;
+            return;
+        }
+        load_run<E>(a.cos_table + (size_t)pos * HALF + sub * E, c);
+        load_run<E>(a.sin_table + (size_t)pos * HALF + sub * E, sn);
+    }
+    long long place = 0;
+    if (!k.queries) {
+        place = place_of(p, a, a.tok_seq[k.t], pos);
+        if (place < 0) return;
+        place += (long long)(is_v ? k.first - p.n_kv : k.first) * p.page_size;
+    }
+    finish_row<HD, TW>(p, a, x, y, w0, w1, c, sn, turns, is_v, k.queries ? (__nv_bfloat16*)a.q_out + ((size_t)k.t * a.n_q + k.first) * HD : nullptr, in, pos, place,
+                       sub, mask);
+}
+
+constexpr int STREAM_R = 4;
+template <int HD>
+struct Stream8 {  // a warp's two places: sixteen rows and a row of the rotation, each piece where the lane that copies it reads it
+    unsigned char rows[4][2][STREAM_R][2][32][HD / 8];
+    float turn[4][2][2][32][HD / 16];
+};
+template <int BYTES>
+__device__ __forceinline__ void copy_own(void* to, const void* from) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (BYTES == 8) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(from) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES; i += 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i), "l"((const char*)from + i) : "memory");
+    }
+}
+
+template <int HD, typename TW>
+__global__ void __launch_bounds__(128, 4) write8_stream_kernel(const GkPages8 p, const Write8 a, int q_tasks, int tasks, unsigned n_tasks) {
+    constexpr int E = HD / 16, HALF = HD / 2;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Stream8<HD>& sm = *reinterpret_cast<Stream8<HD>*>(smem_raw);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7, lane_row = lane >> 3;
+    const unsigned mask = 0xffu << (lane & 24), stride = gridDim.x * 4;
+    unsigned task = blockIdx.x * 4 + warp;
+    if (task >= n_tasks) return;
+    const unsigned kv_tasks = (unsigned)(tasks - q_tasks), kv_all = kv_tasks * (unsigned)a.n_tokens;
+    const auto token = [&](unsigned k) { return k < kv_all ? k / kv_tasks : (k - kv_all) / (unsigned)q_tasks; };
+    const auto position = [&](unsigned k) { return k < n_tasks ? a.tok_pos[token(k)] : 0; };
+    // where a token's keys and values go takes three loads one behind another: each is asked for a task ahead of the next
+    const auto sequence = [&](unsigned k) { return k < kv_all ? a.tok_seq[token(k)] : -1; };
+    const auto slot_in = [&](int seq) { return (unsigned)seq < (unsigned)a.n_seqs ? a.slots[seq] : -1; };
+    const auto page_in = [&](int slot, int pos) {
+        const unsigned index = (unsigned)pos / (unsigned)p.page_size;
+        return (unsigned)slot < (unsigned)p.n_slots && pos >= 0 && index < (unsigned)p.max_pages ? p.table[(size_t)slot * p.max_pages + index] : -1;
+    };
+    const auto ask = [&](unsigned which, int pos, int to) {
+        if (which < n_tasks) {
+            const Task8 k = task_of<HD, STREAM_R>(p, a, which, q_tasks, tasks, lane_row);
+#pragma unroll
+            for (int j = 0; j < STREAM_R; ++j) {
+                const __nv_bfloat16* row = k.in + (size_t)min(k.first + 4 * j, k.n_rows - 1) * HD + sub * E;
+                copy_own<HD / 8>(sm.rows[warp][to][j][0][lane], row);
+                copy_own<HD / 8>(sm.rows[warp][to][j][1][lane], row + HALF);
+            }
+            if (a.cos_table && (unsigned)pos < (unsigned)a.table_positions) {
+                copy_own<HD / 4>(sm.turn[warp][to][0][lane], a.cos_table + (size_t)pos * HALF + sub * E);
+                copy_own<HD / 4>(sm.turn[warp][to][1][lane], a.sin_table + (size_t)pos * HALF + sub * E);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int pos = position(task), pos_next = position(task + stride), seq_2 = sequence(task + 2 * stride);
+    int slot_next = slot_in(sequence(task + stride)), page = page_in(slot_in(sequence(task)), pos);
+    ask(task, pos, 0);
+    float w0[E], w1[E];
+    bool weights_of_queries = false, weights = false;
+    for (int in_hand = 0; task < n_tasks; task += stride, in_hand ^= 1) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");  // a lane reads only what it has copied itself
+        ask(task + stride, pos_next, in_hand ^ 1);
+        const int pos_here = pos, page_here = page;
+        page = page_in(slot_next, pos_next);
+        slot_next = slot_in(seq_2);
+        seq_2 = sequence(task + 3 * stride);
+        pos = pos_next;
+        pos_next = position(task + 2 * stride);
+        const Task8 k = task_of<HD, STREAM_R>(p, a, task, q_tasks, tasks, lane_row);
+        const bool turns = a.cos_table != nullptr, known = !turns || (unsigned)pos_here < (unsigned)a.table_positions;
+        const bool placed = k.queries || (unsigned long long)(long long)page_here < (unsigned long long)p.n_pages;
+        if (!(known && placed) && p.error) *p.error = ERR_PLACE;
+        if (!placed) continue;
+        const long long place0 = k.queries ? 0 : (long long)page_here * p.n_kv * p.page_size + pos_here % p.page_size;
+        float c[E], sn[E];
+        if (a.use_norm && (!weights || weights_of_queries != k.queries)) {
+            const TW* w = (const TW*)(k.queries ? a.wq : a.wk) + sub * E;
+            load_run<E>(w, w0);
+            load_run<E>(w + HALF, w1);
+            weights = true;
+            weights_of_queries = k.queries;
+        }
+        if (turns) {
+            load_run<E>(sm.turn[warp][in_hand][0][lane], c);
+            load_run<E>(sm.turn[warp][in_hand][1][lane], sn);
+        }
+#pragma unroll 1
+        for (int j = 0; j < STREAM_R; ++j) {
+            const int row = k.first + 4 * j;
+            const bool is_v = !k.queries && row >= p.n_kv;
+            if (row >= k.n_rows || (!is_v && !known)) continue;
+            float x[E], y[E];
+            load_run<E>(reinterpret_cast<const __nv_bfloat16*>(sm.rows[warp][in_hand][j][0][lane]), x);
+            load_run<E>(reinterpret_cast<const __nv_bfloat16*>(sm.rows[warp][in_hand][j][1][lane]), y);
+            finish_row<HD, TW>(p, a, x, y, w0, w1, c, sn, turns && !is_v, is_v, k.queries ? (__nv_bfloat16*)a.q_out + ((size_t)k.t * a.n_q + row) * HD : nullptr,
+                               k.in + (size_t)row * HD, pos_here, place0 + (long long)(is_v ? row - p.n_kv : row) * p.page_size, sub, mask);
+        }
+    }
+}
+
+template <int HD, typename TW>
+int launch_write8(const GkPages8& p, const Write8& a, cudaStream_t stream) {
+    // Sixteen rows a task would leave the device idle where rows are few: four below eight warps' worth of sixteen an SM.
+    const bool many = (long long)a.n_tokens * (a.n_q + 2 * p.n_kv) >= 148 * 8 * 16;
+    const int per = many ? 4 * STREAM_R : 4, q_tasks = (a.n_q + per - 1) / per, tasks = q_tasks + (a.write_kv ? (2 * p.n_kv + per - 1) / per : 0);
+    const long long n_tasks = (long long)a.n_tokens * tasks, blocks = (n_tasks + 3) / 4;
+    GK_REQUIRE(n_tasks + 148 * 4 * 4 * 3 < 4294967295LL, "write8: too many tokens");
+    if (!many) {
+        gk_launch(write8_wide_kernel<HD, TW>, dim3((unsigned)blocks), dim3(128), 0, stream, p, a, q_tasks, tasks, (unsigned)n_tasks);
+        GK_CHECK_LAUNCH("write8");
+        return GK_OK;
+    }
+    const int smem = (int)sizeof(Stream8<HD>);
+    cudaError_t err = cudaFuncSetAttribute(write8_stream_kernel<HD, TW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return gk_fail(GK_CUDA_ERROR, "write8: %s", cudaGetErrorString(err));
+    gk_launch(write8_stream_kernel<HD, TW>, dim3((unsigned)(blocks < 148 * 4 ? blocks : 148 * 4)), dim3(128), smem, stream, p, a, q_tasks, tasks, (unsigned)n_tasks);
+    GK_CHECK_LAUNCH("write8");
+    return GK_OK;
 }
 
 // ------------------------------------------------------------------ read back
@@ -371,11 +604,8 @@ GK_EXPORT int gk_write8(const GkPages8* pages, const void* qkv, int dtype, const
     if (dtype == GK_BF16 && (pages->head_dim == 64 || pages->head_dim == 128) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)wq | (uintptr_t)wk |
                                                                                   (uintptr_t)cos_table | (uintptr_t)sin_table) & 15) == 0) {
         GK_DISPATCH_DTYPE(weight_dtype, TW, {
-            if (pages->head_dim == 64) gk_launch(write8_wide_kernel<64, TW>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, *pages, a);
-            else gk_launch(write8_wide_kernel<128, TW>, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, *pages, a);
+            return pages->head_dim == 64 ? launch_write8<64, TW>(*pages, a, (cudaStream_t)stream) : launch_write8<128, TW>(*pages, a, (cudaStream_t)stream);
         })
-        GK_CHECK_LAUNCH("write8");
-        return GK_OK;
     }
     GK_DISPATCH_DTYPE(dtype, T, {
         GK_DISPATCH_DTYPE(weight_dtype, TW, {

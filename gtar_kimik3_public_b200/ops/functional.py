@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .library import KernelError, call, dtype_code, library, ptr, require_device, stream_ptr
+from .library import KernelError, call, current_device, dtype_code, library, ptr, require_device, stream_ptr
 
 
 def _check(tensor: torch.Tensor, name: str, dtype=None, dims: int | None = None) -> None:
@@ -2477,6 +2477,8 @@ class PagedKV8:
                         self.block_table.shape[0], self.block_table.shape[1], n_kv, page, d)
         object.__setattr__(self, "_pages", pages)
         object.__setattr__(self, "_at", ctypes.addressof(pages))
+        object.__setattr__(self, "_index", self.k.get_device())
+        object.__setattr__(self, "_sizes", (n_pages, n_kv, page, d))
 
     @property
     def page_size(self) -> int:
@@ -2495,15 +2497,16 @@ class Work8:
 
 
 def _check8(kv: PagedKV8, given: torch.Tensor, *ints: tuple[str, torch.Tensor, int]) -> None:
-    """What every call over 8-bit pages asks of its tensors: ``ints`` are (name, int32 tensor, entries or -1)."""
-    device = kv.k.device
-    if given.device != device:
-        raise KernelError(f"the tensors are on {given.device}, the pages on {device}")
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"the pages are on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+    """What every call over 8-bit pages asks of its tensors: ``ints`` are (name, int32 tensor, entries or -1).  (Device numbers and not
+    ``torch.device``: a call of few microseconds is asked for in as many.)"""
+    index = kv._index
+    if given.get_device() != index:
+        raise KernelError(f"the tensors are on {given.device}, the pages on {kv.k.device}")
+    if current_device() != index:
+        raise KernelError(f"the pages are on {kv.k.device}, but the current device is cuda:{current_device()}")
     for name, t, entries in ints:
-        if t.dtype != torch.int32 or t.dim() != 1 or t.device != device or not t.is_contiguous():
-            raise KernelError(f"{name} must be a contiguous int32 vector on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous():
+            raise KernelError(f"{name} must be a contiguous int32 vector on {kv.k.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         if entries >= 0 and t.shape[0] != entries:
             raise KernelError(f"{name} must have {entries} entries, got {t.shape[0]}")
 
@@ -2520,9 +2523,9 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
     code = dtype_code(qkv.dtype)
     if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
         raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
-    if kv.k.shape[1] != n_kv or kv.k.shape[3] != head_dim:
+    if kv._sizes[1] != n_kv or kv._sizes[3] != head_dim:
         raise KernelError(f"pages {tuple(kv.k.shape)} do not fit n_kv={n_kv}, head_dim={head_dim}")
-    weight_code = 0
+    weight_code = table_positions = 0
     if (q_weight is None) != (k_weight is None):
         raise KernelError("q and k are normed both or neither")
     if q_weight is not None:
@@ -2531,7 +2534,6 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
         if q_weight.shape[0] != head_dim or k_weight.shape[0] != head_dim:
             raise KernelError("q/k norm weights must have head_dim entries")
         weight_code = dtype_code(q_weight.dtype)
-    table_positions = 0
     if (cos is None) != (sin is None):
         raise KernelError("cos and sin tables go together")
     if cos is not None:
@@ -2542,9 +2544,10 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
         table_positions = cos.shape[0]
     if q_out is None:
         q_out = torch.empty((n, n_q, head_dim), dtype=qkv.dtype, device=qkv.device)
-    _check(q_out, "q_out", qkv.dtype, 3)
-    if q_out.shape != (n, n_q, head_dim):
-        raise KernelError(f"q_out is {tuple(q_out.shape)}, expected {(n, n_q, head_dim)}")
+    else:
+        _check(q_out, "q_out", qkv.dtype, 3)
+        if q_out.shape != (n, n_q, head_dim):
+            raise KernelError(f"q_out is {tuple(q_out.shape)}, expected {(n, n_q, head_dim)}")
     call("gk_write8", kv._at, ptr(qkv), code, ptr(q_weight), ptr(k_weight), weight_code, int(q_weight is not None), float(eps), ptr(cos), ptr(sin),
          table_positions, int(max_position), ptr(tok_pos), ptr(tok_seq), ptr(slots), slots.shape[0], ptr(q_out), n, n_q, int(write_kv), stream_ptr())
     return q_out
@@ -2570,13 +2573,18 @@ def read_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_
 def _check_queries8(q: torch.Tensor, kv: PagedKV8, out: torch.Tensor | None) -> torch.Tensor:
     if q.dim() != 3 or not q.is_cuda or not q.is_contiguous():
         raise KernelError(f"q must be a contiguous CUDA tensor [tokens, heads, head size], got {tuple(q.shape)} on {q.device}")
-    if q.shape[2] != kv.k.shape[3] or q.shape[1] % kv.k.shape[1]:
-        raise KernelError(f"queries {tuple(q.shape)} do not fit pages of {kv.k.shape[1]} kv heads of {kv.k.shape[3]}")
+    _, n_kv, _, d = kv._sizes
+    if q.shape[2] != d or q.shape[1] % n_kv:
+        raise KernelError(f"queries {tuple(q.shape)} do not fit pages of {n_kv} kv heads of {d}")
     if out is None:
         return torch.empty_like(q)
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise KernelError(f"out must be like q, {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
     return out
+
+
+def _sm_count_of(index: int) -> int:
+    return _sm_counts[index] if index in _sm_counts else sm_count(torch.device("cuda", index))
 
 
 ROWS8_HEAD_DIMS = (64, 128)
@@ -2621,13 +2629,13 @@ def rows8_cut(pairs: int, kv_len: int, places: tuple[int, int, int, int]) -> tup
 
 def _rows8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor | None, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, kv_len_hint: int,
            scale: float, window: int, sink: bool, cut: tuple[int, int] | None, out: torch.Tensor) -> torch.Tensor:
-    n_seqs, n_q, d = kv_len.shape[0], q.shape[1], q.shape[2]
-    n_kv = kv.k.shape[1]
+    n_seqs, n_q = kv_len.shape[0], q.shape[1]
+    _, n_kv, _, d = kv._sizes
     n_rows = max_q_len * (n_q // n_kv)
     rows = 8 if n_rows <= 8 else 16
     pairs = n_seqs * -(-n_rows // rows) * n_kv
     if cut is None:
-        cut = rows8_cut(pairs, min(kv_len_hint, window + max_q_len) if window else kv_len_hint, rows8_places(d, rows, sm_count(q.device)))
+        cut = rows8_cut(pairs, min(kv_len_hint, window + max_q_len) if window else kv_len_hint, rows8_places(d, rows, _sm_count_of(kv._index)))
     splits, pieces = cut
     scratch = None
     if splits == 0:
@@ -2646,15 +2654,34 @@ def attention_decode8(q: torch.Tensor, kv: PagedKV8, kv_len: torch.Tensor, slots
     out = _check_queries8(q, kv, out)
     n, n_q, d = q.shape
     _check8(kv, q, ("kv_len", kv_len, n), ("slots", slots, n))
-    if q.dtype == torch.bfloat16 and d in ROWS8_HEAD_DIMS and kv.k.shape[2] == 64 and n_q // kv.k.shape[1] <= ROWS8_MAX_GROUP:
+    _, n_kv, page, _ = kv._sizes
+    if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and n_q // n_kv <= ROWS8_MAX_GROUP:
         return _rows8(q, kv, None, kv_len, slots, 1, max_kv_len, scale, window, sink, cut, out)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), None, ptr(kv_len), ptr(slots), n, n, n_q, float(scale), int(window), int(sink),
          stream_ptr())
     return out
 
 
-# Rows (tokens x query heads of a kv head) of a sequence up to which several tokens go through the kernel for few rows.
-ROWS8_PROMPT_MAX = 64
+@functools.lru_cache(maxsize=4096)
+def rows8_wins(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, n_kv: int, group: int, d: int, sm_count: int) -> bool:
+    """Whether several tokens a sequence go through the kernel for few rows (16 at a time, every tile reading its keys by itself) and not through pages
+    made bfloat16 and the prefill attention (128 rows a tile on tcgen05 for heads of 128, 64 through mma for heads of 64).
+
+    Estimates in us.  Few rows: 650 steps of 32 keys a us with heads of 128 and 1,000 with heads of 64, ten steps' worth besides for each (tile, kv
+    head), and 0.003 for each block of the launch, the empty ones of shorter sequences too.  Prefill: pages at 5.5 TB/s, and the longer of the chain of one
+    tile (1.3 a 128 keys, 1.9 with heads of 64) and the tiles' chains over the SMs.  Measured, few rows / prefill, 32/8 heads of 128: 16 sequences of 4
+    tokens behind 2,000 23 / 68, of 16 tokens 59 / 69, of 32 tokens 111 / 70; one of 64 behind 4,000 30 / 49, of 512 behind 2,000 117 / 37; prompts of
+    128, 256, 512: 8.6 / 11.4, 17 / 12.6, 37 / 15.9; 12/4 heads of 64: 8 of 32 behind 4,000 35 / 72, prompts of 1,024 and 2,048 26 / 25 and 67 / 46."""
+    tiles = n_tokens * group // 16 + n_seqs
+    launched = n_seqs * -(-max_q_len * group // 16) * n_kv
+    if launched // n_kv > 65535:
+        return False
+    middle = max(1, max_kv_len - max_q_len // 2)
+    rows = 5 + min(tiles * n_kv, launched) * (middle / 32 + 10) / (650 if d == 128 else 1000) + 0.003 * launched
+    step = (1.3 if d == 128 else 1.9) / 128
+    blocks = (n_tokens * group // 128 + n_seqs) * n_kv
+    prefill = 10 + n_seqs * max_kv_len * n_kv * 6 * d / 5.5e6 + max(max_kv_len * step, blocks / sm_count * middle * step)
+    return rows < prefill
 
 
 def _clean_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, last: int) -> tuple[PagedKV, torch.Tensor, torch.Tensor]:
@@ -2680,9 +2707,11 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     out = _check_queries8(q, kv, out)
     n_seqs = kv_len.shape[0]
     _check8(kv, q, ("cu_q", cu_q, n_seqs + 1), ("kv_len", kv_len, n_seqs), ("slots", slots, n_seqs))
-    group = q.shape[1] // kv.k.shape[1]
-    if q.dtype == torch.bfloat16 and q.shape[2] in ROWS8_HEAD_DIMS and kv.k.shape[2] == 64 and group <= ROWS8_MAX_GROUP and n_seqs and q.shape[0]:
-        if max_q_len * group <= ROWS8_PROMPT_MAX:
+    n_tokens, n_q, d = q.shape
+    _, n_kv, page, _ = kv._sizes
+    group = n_q // n_kv
+    if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and group <= ROWS8_MAX_GROUP and n_seqs and n_tokens:
+        if rows8_wins(n_tokens, n_seqs, max_q_len, min(max_kv_len, window + max_q_len) if window else max_kv_len, n_kv, group, d, _sm_count_of(kv._index)):
             return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
         pages, lens, own_slots = _clean_pages8(kv, kv_len, slots, max_kv_len, window + max_q_len if window else 0)
         return attention_prefill(q, pages, cu_q, lens, own_slots, max_q_len, scale, window, out, sink=sink)

@@ -114,6 +114,46 @@ def test_write(dtype, n_q, n_kv, d, norm, rope):
         assert (getattr(kv, name + "_exp").cpu()[untouched] == 255).all()
 
 
+@pytest.mark.parametrize("n_q,n_kv,d,lens", [(16, 8, 128, [700, 1, 65]), (6, 2, 64, [1500, 800]), (3, 3, 128, [2300])])
+@pytest.mark.parametrize("norm", [True, False])
+def test_write_of_many_tokens(n_q, n_kv, d, lens, norm):
+    """Enough rows for the warps that stay.  Keys are the formula in 64 bits rounded once, all of them; a place outside the pages is left out and
+    reported, the others are what they are."""
+    past, eps = [5 * i for i in range(len(lens))], 1e-6
+    kv, slots, table = empty_pages(len(lens), max(lens) + 20, n_kv, d)
+    pos = [p + i for n, p in zip(lens, past) for i in range(n)]
+    seq = [i for i, n in enumerate(lens) for _ in range(n)]
+    qkv = rand(len(pos), (n_q + 2 * n_kv) * d, seed=2).to(torch.bfloat16)
+    assert len(pos) * (n_q + 2 * n_kv) >= 148 * 8 * 16
+    wq, wk = (1 + 0.1 * rand(d, seed=20)).to(torch.bfloat16), (1 + 0.1 * rand(d, seed=21)).to(torch.bfloat16)
+    cos, sin = plain.rotary_tables(torch.arange(max(pos) + 1), d, 1e4)
+    cos, sin = cos[:, : d // 2].float().contiguous(), sin[:, : d // 2].float().contiguous()
+    wrong = len(pos) // 2
+    seq_given = list(seq)
+    seq_given[wrong] = len(lens)
+    args = (wq.to(DEV), wk.to(DEV), eps, cos.to(DEV), sin.to(DEV)) if norm else (None, None, eps, None, None)
+    q = F().qk_norm_rope_write8(qkv.to(DEV), n_q, n_kv, d, *args, ints(*pos), ints(*seq_given), slots, kv, max(pos))
+    with pytest.raises(Exception, match="page number"):
+        F().check_kernel_errors(DEV)
+    x = qkv.double().view(-1, n_q + 2 * n_kv, d)
+
+    def finished(y, w):
+        if not norm:
+            return y
+        c, s = (torch.cat([t[pos], t[pos]], -1).double() for t in (cos, sin))
+        return plain.apply_rotary(plain.rms_norm(y, w.double(), eps), c, s)
+
+    want_q, want_k, want_v = finished(x[:, :n_q], wq), finished(x[:, n_q:n_q + n_kv], wk), x[:, n_q + n_kv:]
+    reach = want_q.abs().amax(-1, keepdim=True)
+    assert ((q.double().cpu() - want_q).abs() <= 2.0**-8 * want_q.abs() + (2.0**-20 if norm else 0) * reach).all()
+    want_k, want_v = plain8.quantised(want_k), plain8.quantised(want_v)
+    got = [held(kv, table, int(slots[i]), p + n) for i, (n, p) in enumerate(zip(lens, past))]
+    got_k, got_v = (torch.cat([g[j][p:] for g, p in zip(got, past)]) for j in (0, 1))
+    keep = torch.arange(len(pos)) != wrong
+    assert torch.equal(got_v[keep], want_v[keep]) and torch.equal(got_k[keep], want_k[keep])
+    assert torch.isnan(got_k[wrong]).all()  # the poison
+
+
 @pytest.mark.parametrize("d", [32, 64, 128])
 def test_write_rows_at_the_edges(d):
     """Zeros, a maximum of 448 times a power and right above it, ties between two numbers, numbers below the smallest step, the largest and
@@ -227,11 +267,13 @@ def test_decode(dtype, cut, n_q, n_kv, d, window, sink):
     F().check_kernel_errors(DEV)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dtype,few", [(torch.bfloat16, None), (torch.bfloat16, True), (torch.bfloat16, False), (torch.float32, None)])
 @pytest.mark.parametrize("n_q,n_kv,d", GROUPS)
 @pytest.mark.parametrize("window,sink", [(0, False), (70, True)])
 @pytest.mark.parametrize("new,lens", [([4, 1, 7, 3], [4, 200, 71, 66]), ([150, 1, 65, 0, 90], [150, 130, 300, 64, 90])])
-def test_prefill(dtype, n_q, n_kv, d, window, sink, new, lens):
+def test_prefill(dtype, few, n_q, n_kv, d, window, sink, new, lens, monkeypatch):
+    if few is not None:  # through the kernel for few rows, or through clean pages, whichever the rule would take
+        monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: few)
     kv, slots, table = sequences(lens, n_kv, d, window=window, new=new)
     cu = [0]
     for n in new:
@@ -289,8 +331,10 @@ def test_numbers_that_are_none(n_q, n_kv, d):
 @pytest.mark.parametrize("n_q,n_kv,d", [(4, 2, 128), (6, 2, 64), (6, 2, 80)])
 @pytest.mark.parametrize("m", [5, 90])
 @pytest.mark.parametrize("window", [0, 40])
-def test_values_that_are_none_reach_only_who_sees_them(n_q, n_kv, d, m, window):
+@pytest.mark.parametrize("few", [True, False])
+def test_values_that_are_none_reach_only_who_sees_them(n_q, n_kv, d, m, window, few, monkeypatch):
     """A value that holds a NaN: tokens in front of it, tokens whose window has left it and other heads do not meet it."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: few)
     n, group = 150, n_q // n_kv
     kv, slots, table = sequences([n, 80], n_kv, d)
     at = n - m + 2  # the step's third token
@@ -306,8 +350,9 @@ def test_values_that_are_none_reach_only_who_sees_them(n_q, n_kv, d, m, window):
     assert torch.isnan(got[:m, group:2 * group][see][:, :, 7]).all()
 
 
-def test_prefill_where_pages_keep_their_numbers():
-    """Bounds on lengths so large that renumbered pages would be more than there are."""
+def test_prefill_where_pages_keep_their_numbers(monkeypatch):
+    """Bounds on lengths so large that renumbered pages would be more than there are: the prefill kernels see the same pages under other numbers."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: False)
     n_q, n_kv, d, new, lens = 4, 2, 128, [70, 1, 40], [200, 64, 40]
     kv, slots, table = sequences(lens, n_kv, d, new=new)
     wide = torch.cat([kv.block_table, torch.zeros((kv.block_table.shape[0], 60), dtype=torch.int32, device=DEV)], 1).contiguous()
@@ -319,8 +364,10 @@ def test_prefill_where_pages_keep_their_numbers():
     F().check_kernel_errors(DEV)
 
 
-def test_page_numbers_slots_and_lengths_that_cannot_be():
+@pytest.mark.parametrize("few", [True, False])
+def test_page_numbers_slots_and_lengths_that_cannot_be(few, monkeypatch):
     """They are skipped and reported; the step's other sequences are what they are."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: few)
     n_q, n_kv, d = 4, 2, 128
     lens = [100, 90, 70]
     kv, slots, table = sequences(lens, n_kv, d)
