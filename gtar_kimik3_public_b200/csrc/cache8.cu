@@ -178,27 +178,31 @@ __device__ __forceinline__ void load_run<8, float>(const float* from, float (&v)
     }
 }
 
-// A key in 64 bits, by the eight lanes of its row.
+// A key in 64 bits, or a row of values that holds an infinity, by the eight lanes of its row.
 template <int HD, typename TW>
-__device__ __noinline__ void write_key_64(const GkPages8& p, const Write8& a, const __nv_bfloat16* row, int pos, long long place, int sub, unsigned mask) {
+__device__ __noinline__ void write_row_with_care(const GkPages8& p, const Write8& a, const __nv_bfloat16* row, bool is_v, int pos, long long place, int sub,
+                                                 unsigned mask) {
     constexpr int E = HD / 16, HALF = HD / 2;
     const auto at = [&](int i) { return sub * E + i; };
     float x[E], y[E];
-    double u[E], v[E];
     load_run<E>(row + sub * E, x);
     load_run<E>(row + HALF + sub * E, y);
+    if (!is_v) {
+        double u[E], v[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) u[i] = x[i], v[i] = y[i];
-    norm_rotate(u, v, a, (const TW*)a.wk, HALF, pos, 8, mask, at);
+        for (int i = 0; i < E; ++i) u[i] = x[i], v[i] = y[i];
+        norm_rotate(u, v, a, (const TW*)a.wk, HALF, pos, 8, mask, at);
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
-    store_bytes(x, y, p.k + place * HD, p.k_exp + place, HALF, 8, mask, sub == 0, at);
+        for (int i = 0; i < E; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
+    }
+    store_bytes(x, y, (is_v ? p.v : p.k) + place * HD, (is_v ? p.v_exp : p.k_exp) + place, HALF, 8, mask, sub == 0, at);
 }
 
-// Whether `y`, scaled and rounded to `got`, lies within `tol` of the middle between two e4m3 numbers.
-__device__ __forceinline__ bool near_middle(float y, float got, float tol) {
-    const uint32_t power = max(__float_as_uint(fabsf(y)) & 0x7f800000u, 0x3c800000u);  // 2^-6 at the least
-    return __uint_as_float(power - (4u << 23)) - fabsf(y - got) < tol;
+// Two finite numbers, scaled already, as e4m3: `lo` in the low byte.
+__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 template <int E>
@@ -256,34 +260,47 @@ __device__ __forceinline__ void finish_row(const GkPages8& p, const Write8& a, f
     }
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
+    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(y[i])));  // (passes over NaN)
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
     const int b = exponent_byte(top);
     const float back = power_back(b);
     uint32_t four[2][E / 4];
-    bool unsure = abs((int)(__float_as_uint(top) & 0x7fffffu) - 0x600000) < 32;  // 2^-18 of the border between two powers
+    bool care = top == INFINITY;
+    if (is_v || !(a.use_norm || turns)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < E; i += 4)
+                four[h][i / 4] = pack2_finite((h ? y : x)[i] * back, (h ? y : x)[i + 1] * back) | pack2_finite((h ? y : x)[i + 2] * back, (h ? y : x)[i + 3] * back) << 16;
+    } else {
+        // Off by 1.5 * 2^-21 of itself at most through the norm's factor, and by 2^-21 of both numbers that the rotation mixes through the roundings of
+        // their products: where as much less and as much more are not the same byte, or the maximum lies within 2^-18 of the next power's, the row
+        // is made over.
+        care |= abs((int)(__float_as_uint(top) & 0x7fffffu) - 0x600000) < 32;
+        const float slack = 1.25e-6f * back;
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
-            const float u[4] = {(h ? y : x)[i] * back, (h ? y : x)[i + 1] * back, (h ? y : x)[i + 2] * back, (h ? y : x)[i + 3] * back};
-            const uint32_t lo = pack2(u[0], u[1]), hi = pack2(u[2], u[3]);
-            four[h][i / 4] = lo | hi << 16;
-            if (!is_v) {
-                const float2 g0 = floats2((uint16_t)lo), g1 = floats2((uint16_t)hi);
-                const float got[4] = {g0.x, g0.y, g1.x, g1.y};
+            uint32_t less[2][2], more[2][2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // 1.5 * 2^-21 of the number for the norm's factor, 2^-22 of both numbers that the rotation mixes for the roundings of its
-                    // products, twice
-                    const float other = fabsf((h ? x : y)[i + e] * back);
-                    unsure |= near_middle(u[e], got[e], fmaf(4.76837158e-7f, other, 1.19209290e-6f * fabsf(u[e])));
+            for (int e = 0; e < 4; e += 2) {
+                const float t0 = slack * (fabsf(x[i + e]) + fabsf(y[i + e])), t1 = slack * (fabsf(x[i + e + 1]) + fabsf(y[i + e + 1]));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float u = (h ? y : x)[i + e], v = (h ? y : x)[i + e + 1];
+                    less[h][e / 2] = pack2_finite(fmaf(u, back, -t0), fmaf(v, back, -t1));
+                    more[h][e / 2] = pack2_finite(fmaf(u, back, t0), fmaf(v, back, t1));
                 }
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                four[h][i / 4] = less[h][0] | less[h][1] << 16;
+                care |= four[h][i / 4] != (more[h][0] | more[h][1] << 16);
+            }
         }
-    if (!is_v && (a.use_norm || turns) && __any_sync(mask, unsure)) {
-        write_key_64<HD, TW>(p, a, in, pos, place, sub, mask);
+    }
+    if (__any_sync(mask, care)) {
+        write_row_with_care<HD, TW>(p, a, in, is_v, pos, place, sub, mask);
         return;
     }
     uint8_t* to = (is_v ? p.v : p.k) + place * HD + sub * E;
