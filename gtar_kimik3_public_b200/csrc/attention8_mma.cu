@@ -25,7 +25,7 @@
 
 #include <atomic>
 
-#include "cache8.cuh"
+#include "cache8_write.cuh"
 
 namespace {
 
@@ -44,6 +44,14 @@ struct Rows8 {
     int n_splits;  // blocks of a cluster that share a (unit, kv head); 0: pieces of one size, about `pieces` of them
     int pieces;
     float *part_o, *part_abl;  // of pieces: [piece][row][D] and [piece][row][A, B, l]
+};
+
+// A step of one token a sequence that does its input stage too: `qkv` [n_seqs][(n_q + 2 n_kv) * D] is the packed projection; queries are normed and
+// rotated here, and (`write_kv`) the new key and value put into the cache, by the warp that has the tile they lie in: it also puts their bytes into that
+// tile's copy in shared memory, which is asked for without them.
+struct Fused8 : Norm8 {
+    const __nv_bfloat16* qkv;
+    int weights_bf16, write_kv;
 };
 
 // A unit: which rows, which tokens, and the keys that some or all of them see.
@@ -191,7 +199,8 @@ struct Smem8 {
         float o[WARPS][ROWS * STRIDE];  // what a warp has of its rows, in the end
     };
     float abl[WARPS][ROWS][3];
-    float from_o[ROWS * D + 8 * 4];  // from the other blocks of a cluster: [block][place] of four numbers
+    unsigned char fresh[2][D], fresh_power[2];  // bytes of the new key and value
+    alignas(16) float from_o[ROWS * D + 8 * 4];  // from the other blocks of a cluster: [block][place] of four numbers
     float from_abl[8][ROWS][3];
 };
 
@@ -215,12 +224,105 @@ __device__ __forceinline__ void store4(__nv_bfloat16* to, const float4& v, float
 
 // A block's share of one (unit, kv head): the tiles tile_begin .. tile_end - 1.  `part` < 0: the whole of it or a cluster's split; else where its
 // sums go.
-template <int D, int NT>
-__device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, Smem8<D, NT>& sm, const Unit& u, int hk, int tile_begin, int tile_end, int split,
+// RMSNorm and rotation of a query whose columns 64 c + 16 t .. + 15 lane t of a quad holds.
+template <int D>
+__device__ __forceinline__ void norm_rotate_queries(const Fused8& f, float (&x)[D / 64][16], int pos, int t) {
+    if (f.use_norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ss += x[c][i] * x[c][i];
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+        const float inv = rsqrtf(fmaf(ss, 1.f / D, f.eps));
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; i += 8) {
+                float w[8];
+                if (f.weights_bf16) load_run<8>((const __nv_bfloat16*)f.wq + 64 * c + 16 * t + i, w);
+                else load_run<8>((const float*)f.wq + 64 * c + 16 * t + i, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][i + e] = (x[c][i + e] * inv) * w[e];
+            }
+    }
+    if (f.cos_table && (unsigned)pos < (unsigned)f.table_positions) {
+        const size_t at = (size_t)pos * (D / 2) + (D == 128 ? 16 * t : 16 * (t & 1));
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+            float c[8], s[8];
+            load_run<8>(f.cos_table + at + i, c);
+            load_run<8>(f.sin_table + at + i, s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (D == 128) {
+                    const float u = x[0][i + e], v = x[D / 64 - 1][i + e];
+                    x[0][i + e] = u * c[e] - v * s[e];
+                    x[D / 64 - 1][i + e] = v * c[e] + u * s[e];
+                } else {  // the other half lies with lane t ^ 2
+                    const float u = x[0][i + e], v = __shfl_xor_sync(0xffffffffu, u, 2);
+                    x[0][i + e] = t < 2 ? u * c[e] - v * s[e] : u * c[e] + v * s[e];
+                }
+            }
+        }
+    }
+}
+
+// The new key and value of a sequence: lanes 0 .. 7 the key, 8 .. 15 the value.
+template <int D, typename TW>
+__device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, const Fused8& f, const Unit& u, int hk, int lane, unsigned char (&bytes)[2][D],
+                                         unsigned char (&powers)[2]) {
+    constexpr int E = D / 16, HALF = D / 2;
+    const int sub = lane & 7, pos = u.past;
+    const bool is_v = lane >= 8;
+    const unsigned mask = 0xffu << (lane & 24);
+    if (lane < 16) {
+        const __nv_bfloat16* row = f.qkv + ((size_t)u.first_token * (a.n_q + 2 * p.n_kv) + a.n_q + (is_v ? p.n_kv : 0) + hk) * D;
+        float x[E], y[E], w0[E], w1[E], c[E], sn[E];
+        load_run<E>(row + sub * E, x);
+        load_run<E>(row + HALF + sub * E, y);
+        const bool turns = f.cos_table != nullptr && !is_v && (unsigned)pos < (unsigned)f.table_positions;
+        if (f.cos_table != nullptr && (unsigned)pos >= (unsigned)f.table_positions && p.error) *p.error = ERR_PLACE;
+        if (!is_v) {
+            if (f.use_norm) {
+                load_run<E>((const TW*)f.wk + sub * E, w0);
+                load_run<E>((const TW*)f.wk + HALF + sub * E, w1);
+            }
+            if (turns) {
+                load_run<E>(f.cos_table + (size_t)pos * HALF + sub * E, c);
+                load_run<E>(f.sin_table + (size_t)pos * HALF + sub * E, sn);
+            }
+            norm_rotate_32<D>(f, x, y, w0, w1, c, sn, turns, mask);
+        }
+        uint32_t four[2][E / 4];
+        const int b = make_bytes<D, TW>(f, x, y, turns, is_v, row, pos, sub, mask, four);
+        const int page = page_of(p, u.slot, pos / PAGE);
+        const size_t place = ((size_t)max(page, 0) * p.n_kv + hk) * PAGE + pos % PAGE;
+        uint8_t* to = (is_v ? p.v : p.k) + place * D + sub * E;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) {
+                *reinterpret_cast<uint32_t*>(&bytes[is_v][h * HALF + sub * E + 4 * i]) = four[h][i];
+                if (page >= 0) *reinterpret_cast<uint32_t*>(to + h * HALF + 4 * i) = four[h][i];
+            }
+        if (sub == 0) {
+            powers[is_v] = (unsigned char)b;
+            if (page >= 0) (is_v ? p.v_exp : p.k_exp)[place] = (uint8_t)b;
+        }
+    }
+    __syncwarp();
+}
+
+template <int D, int NT, bool FUSED>
+__device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const Fused8& f, Smem8<D, NT>& sm, const Unit& u, int hk, int tile_begin, int tile_end, int split,
                                       int part) {
     constexpr int ROWS = 8 * NT, KS = D / 16, MT = D / 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n_rows = u.n_rows, row_first = u.row_first, first_token = u.first_token, past = u.past, begin = u.begin, end = u.end;
+    const int n_rows = u.n_rows, row_first = u.row_first, first_token = u.first_token, past = u.past, begin = u.begin;
+    const bool writes = FUSED && f.write_kv;
+    const int end = u.end - (writes ? 1 : 0);  // the new key's place is not read
 
     // the numbers of the pages of this warp's next 32 tiles, one a lane
     int at = tile_begin + warp;
@@ -250,6 +352,13 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, Smem8<D
     pdl_wait();
     if (!early) ask_next();
 
+    const int new_tile = writes ? past / KEYS : -1;
+    const bool owns = writes && past >= 0 && new_tile >= tile_begin && new_tile < tile_end && (new_tile - tile_begin) % WARPS == warp;
+    if (owns) {
+        if (f.weights_bf16) new_rows<D, __nv_bfloat16>(p, a, f, u, hk, lane, sm.fresh, sm.fresh_power);
+        else new_rows<D, float>(p, a, f, u, hk, lane, sm.fresh, sm.fresh_power);
+    }
+
     // queries: lane (g, t) has of row g of each tile of eight the columns 64 c + 16 t .. + 15
     uint32_t qf[NT][KS][2];
     float factor[NT][2];  // of the rows 2t, 2t + 1: what a product of halves times a key's power makes a score in powers of two
@@ -262,19 +371,25 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, Smem8<D
         for (int c = 0; c < D / 64; ++c) {
             uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
             if (r < n_rows) {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)(first_token + row / a.group) * a.n_q + hk * a.group + row % a.group) * D + 64 * c + 16 * t);
+                const __nv_bfloat16* q = FUSED ? f.qkv + ((size_t)first_token * (a.n_q + 2 * p.n_kv) + hk * a.group + row) * D
+                                               : a.q + ((size_t)(first_token + row / a.group) * a.n_q + hk * a.group + row % a.group) * D;
+                const uint4* src = reinterpret_cast<const uint4*>(q + 64 * c + 16 * t);
                 raw[0] = src[0];
                 raw[1] = src[1];
             }
             const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(raw);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float2 f = __bfloat1622float2(pairs[i]);
-                x[c][2 * i] = f.x;
-                x[c][2 * i + 1] = f.y;
-                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                const float2 two = __bfloat1622float2(pairs[i]);
+                x[c][2 * i] = two.x;
+                x[c][2 * i + 1] = two.y;
             }
         }
+        if (FUSED) norm_rotate_queries<D>(f, x, past, t);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[c][i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = max((int)(__float_as_uint(top) >> 23) - 127 - 14, -110);  // the row's largest goes to 2^14 .. 2^15
@@ -318,6 +433,16 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, Smem8<D
         __syncwarp();  // the tile has come for every lane, and every lane is done with the place that is asked into next
         ask_next();
         const int key0 = at * KEYS;
+        if (FUSED && owns && at == new_tile) {  // 4 D / 64 bytes a lane into the tile's copy
+            const int row = past - key0, byte = (lane & 15) * (D / 16);
+            unsigned char* key = sm.ring[warp][place == ring ? 0 : 1];
+#pragma unroll
+            for (int i = 0; i < D / 16; i += 4)
+                *reinterpret_cast<uint32_t*>(key + (lane < 16 ? Place<D>::key(row, byte + i) : Place<D>::value(row, byte + i))) =
+                    *reinterpret_cast<const uint32_t*>(&sm.fresh[lane >> 4][byte + i]);
+            if ((lane & 15) == 0) key[(lane ? At::VE : At::KE) + row] = sm.fresh_power[lane >> 4];
+            __syncwarp();
+        }
         // scores of 32 keys x rows: s[h][n][0], [1] = key 4g + 2h, rows 2t, 2t + 1; [2], [3] = key 4g + 2h + 1
         float s[2][NT][4];
 #pragma unroll
@@ -545,8 +670,8 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, Smem8<D
     }
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) rows8_kernel(const GkPages8 p, const Rows8 a) {
+template <int D, int NT, bool FUSED>
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) rows8_kernel(const GkPages8 p, const Rows8 a, const Fused8 f) {
     constexpr int ROWS = 8 * NT;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem8<D, NT>& sm = *reinterpret_cast<Smem8<D, NT>*>(smem_raw);
@@ -559,7 +684,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) rows8_kernel(const G
         }
         if (a.n_splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // all are here before one stores into another's memory
         const int split = blockIdx.x, per = (u.n_tiles + a.n_splits - 1) / a.n_splits, tile_begin = u.tile_0 + split * per;
-        piece<D, NT>(p, a, sm, u, blockIdx.y, tile_begin, min(tile_begin + per, u.tile_0 + u.n_tiles), split, -1);
+        piece<D, NT, FUSED>(p, a, f, sm, u, blockIdx.y, tile_begin, min(tile_begin + per, u.tile_0 + u.n_tiles), split, -1);
         return;
     }
     const int lane = threadIdx.x & 31, size = piece_size(p, a, ROWS, lane);
@@ -572,7 +697,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) rows8_kernel(const G
     const Unit u = unit_of(p, a, unit, ROWS);
     const int cuts = (u.n_tiles + size - 1) / size, hk = (blockIdx.x - before) / cuts, cut = blockIdx.x - before - hk * cuts;
     const int per = (u.n_tiles + cuts - 1) / cuts, tile_begin = u.tile_0 + cut * per;
-    piece<D, NT>(p, a, sm, u, hk, tile_begin, min(tile_begin + per, u.tile_0 + u.n_tiles), 0, cuts == 1 ? -1 : (int)blockIdx.x);
+    piece<D, NT, FUSED>(p, a, f, sm, u, hk, tile_begin, min(tile_begin + per, u.tile_0 + u.n_tiles), 0, cuts == 1 ? -1 : (int)blockIdx.x);
 }
 
 // The pieces of a pair joined: a block a (row, kv head, unit), its warps take every fourth piece each; pairs of one piece are done already.
@@ -622,9 +747,9 @@ __global__ void __launch_bounds__(THREADS) rows8_join_kernel(const GkPages8 p, c
 template <int D, int NT>
 int places_of(int cluster) {
     const int smem = (int)sizeof(Smem8<D, NT>);
-    cudaError_t err = cudaFuncSetAttribute(rows8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t err = cudaFuncSetAttribute(rows8_kernel<D, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return -(int)err;
-    gk_prepare_kernel((const void*)rows8_kernel<D, NT>);
+    gk_prepare_kernel((const void*)rows8_kernel<D, NT, false>);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster * 1024, 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
@@ -637,27 +762,27 @@ int places_of(int cluster) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int clusters = 0;
-    err = cudaOccupancyMaxActiveClusters(&clusters, rows8_kernel<D, NT>, &cfg);
+    err = cudaOccupancyMaxActiveClusters(&clusters, rows8_kernel<D, NT, false>, &cfg);
     return err == cudaSuccess ? clusters : -(int)err;
 }
 
-template <int D, int NT>
-int launch_rows8(const GkPages8& p, const Rows8& a, cudaStream_t stream) {
+template <int D, int NT, bool FUSED>
+int launch_rows8(const GkPages8& p, const Rows8& a, const Fused8& f, cudaStream_t stream) {
     const int smem = (int)sizeof(Smem8<D, NT>);
     static std::atomic<unsigned long long> configured{0};  // a bit a device (the attribute is the device's)
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
     if (err == cudaSuccess && (device > 63 || !(configured.load() >> device & 1))) {
-        err = cudaFuncSetAttribute(rows8_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        err = cudaFuncSetAttribute(rows8_kernel<D, NT, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (err == cudaSuccess && device <= 63) configured.fetch_or(1ull << device);
     }
     if (err != cudaSuccess) return gk_fail(GK_CUDA_ERROR, "rows8: %s", cudaGetErrorString(err));
     if (a.n_splits > 0) {
-        gk_launch_cluster(rows8_kernel<D, NT>, dim3(a.n_splits, p.n_kv, a.n_units), dim3(THREADS), smem, stream, dim3(a.n_splits, 1, 1), p, a);
+        gk_launch_cluster(rows8_kernel<D, NT, FUSED>, dim3(a.n_splits, p.n_kv, a.n_units), dim3(THREADS), smem, stream, dim3(a.n_splits, 1, 1), p, a, f);
         GK_CHECK_LAUNCH("rows8");
         return GK_OK;
     }
-    gk_launch(rows8_kernel<D, NT>, dim3(a.pieces + a.n_units * p.n_kv), dim3(THREADS), smem, stream, p, a);
+    gk_launch(rows8_kernel<D, NT, FUSED>, dim3(a.pieces + a.n_units * p.n_kv), dim3(THREADS), smem, stream, p, a, f);
     GK_CHECK_LAUNCH("rows8");
     const int rows = (int)min(8LL * NT, (long long)a.group * (a.cu_q ? 8 * NT : 1));
     gk_launch_behind(rows8_join_kernel<D, NT>, dim3(rows, p.n_kv, a.n_units), dim3(THREADS), 0, stream, p, a);
@@ -677,8 +802,8 @@ GK_EXPORT int gk_rows8_places(int head_dim, int rows, int cluster) {
 // Rows taken together: 8 or 16.  `splits` 1 .. 8: so many blocks, a cluster, share a (row tile, kv head); 0: the step's keys are cut into pieces of one
 // size, about `pieces` of them, with (pieces + units * n_kv) * rows * (head_dim + 3) floats of scratch, units = sequences * row tiles a sequence.
 // `q`, `out` [n_tokens][n_q][head_dim] bfloat16.  `max_q_len`: no sequence brings more tokens.
-GK_EXPORT int gk_rows8(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_seqs, int n_q,
-                       int max_q_len, int rows, int splits, int pieces, float* scratch, float scale, int window, int sink, void* stream) {
+static int rows8_entry(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_seqs, int n_q,
+                       int max_q_len, int rows, int splits, int pieces, float* scratch, float scale, int window, int sink, const Fused8& f, void* stream) {
     const int status = cache8::check(pages, "rows8");
     if (status != GK_OK) return status;
     const GkPages8& p = *pages;
@@ -689,13 +814,39 @@ GK_EXPORT int gk_rows8(const GkPages8* pages, const void* q, void* out, const in
     GK_REQUIRE(rows == 8 || rows == 16, "rows8: %d rows a tile", rows);
     GK_REQUIRE(splits >= 0 && splits <= 8 && (splits > 0 || (scratch && pieces > 0)), "rows8: %d splits, %d pieces", splits, pieces);
     if (n_seqs == 0) return GK_OK;
-    GK_REQUIRE(q && out && kv_len && slots, "rows8: an array is missing");
+    GK_REQUIRE((q || f.qkv) && out && kv_len && slots, "rows8: an array is missing");
+    GK_REQUIRE((((uintptr_t)q | (uintptr_t)f.qkv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "rows8: memory must begin on 16-byte boundaries");
     const long long group = n_q / p.n_kv, tiles = cu_q ? (max_q_len * group + rows - 1) / rows : 1, units = tiles * n_seqs;
     GK_REQUIRE(cu_q || (max_q_len == 1 && group <= rows), "rows8: %lld heads a kv head do not fit %d rows", group, rows);
     GK_REQUIRE(units <= 65535 && p.n_kv <= 65535 && pieces + units * p.n_kv < 2147483647LL, "rows8: grid too large");
     const Rows8 a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, cu_q, kv_len, slots, n_q, (int)group, (int)tiles, (int)units, scale * 1.4426950408889634f,
                      window, sink, splits, pieces, scratch, scratch ? scratch + (size_t)(pieces + units * p.n_kv) * rows * p.head_dim : nullptr};
     cudaStream_t s = (cudaStream_t)stream;
-    if (p.head_dim == 64) return rows == 8 ? launch_rows8<64, 1>(p, a, s) : launch_rows8<64, 2>(p, a, s);
-    return rows == 8 ? launch_rows8<128, 1>(p, a, s) : launch_rows8<128, 2>(p, a, s);
+    if (f.qkv) {
+        if (p.head_dim == 64) return rows == 8 ? launch_rows8<64, 1, true>(p, a, f, s) : launch_rows8<64, 2, true>(p, a, f, s);
+        return rows == 8 ? launch_rows8<128, 1, true>(p, a, f, s) : launch_rows8<128, 2, true>(p, a, f, s);
+    }
+    if (p.head_dim == 64) return rows == 8 ? launch_rows8<64, 1, false>(p, a, f, s) : launch_rows8<64, 2, false>(p, a, f, s);
+    return rows == 8 ? launch_rows8<128, 1, false>(p, a, f, s) : launch_rows8<128, 2, false>(p, a, f, s);
+}
+
+GK_EXPORT int gk_rows8(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_seqs, int n_q,
+                       int max_q_len, int rows, int splits, int pieces, float* scratch, float scale, int window, int sink, void* stream) {
+    return rows8_entry(pages, q, out, cu_q, kv_len, slots, n_seqs, n_q, max_q_len, rows, splits, pieces, scratch, scale, window, sink, Fused8{}, stream);
+}
+
+// One token a sequence, from the packed projection `qkv` [n_seqs][(n_q + 2 n_kv) * head_dim] bfloat16: norm and rotation of queries and keys and the
+// write of the new key and value (`write_kv`) happen inside.
+GK_EXPORT int gk_rows8_fused(const GkPages8* pages, const void* qkv, const void* wq, const void* wk, int weight_dtype, int use_norm, float eps,
+                             const float* cos_table, const float* sin_table, int table_positions, int max_position, int write_kv, void* out,
+                             const int* kv_len, const int* slots, int n_seqs, int n_q, int rows, int splits, int pieces, float* scratch, float scale,
+                             int window, void* stream) {
+    GK_REQUIRE(qkv || n_seqs == 0, "rows8_fused: qkv is missing");
+    GK_REQUIRE(GK_VALID_DTYPE(weight_dtype) && (!use_norm || (wq && wk)), "rows8_fused: norm weights missing or of a bad type");
+    GK_REQUIRE((cos_table == nullptr) == (sin_table == nullptr), "rows8_fused: cos and sin tables go together");
+    GK_REQUIRE(cos_table == nullptr || max_position < table_positions, "rows8_fused: position %d is beyond the rotary table (%d positions)", max_position,
+               table_positions);
+    GK_REQUIRE((((uintptr_t)wq | (uintptr_t)wk | (uintptr_t)cos_table | (uintptr_t)sin_table) & 15) == 0, "rows8_fused: weights and tables must begin on 16-byte boundaries");
+    const Fused8 f = {{wq, wk, cos_table, sin_table, table_positions, use_norm, eps}, (const __nv_bfloat16*)qkv, weight_dtype == GK_BF16, write_kv};
+    return rows8_entry(pages, nullptr, out, nullptr, kv_len, slots, n_seqs, n_q, 1, rows, splits, pieces, scratch, scale, window, 0, f, stream);
 }

@@ -7,58 +7,19 @@
 // 128: 50 us more), so the wide kernel makes them in 32 bits and does over, in 64, the rows that have a number or their maximum next to a border:
 // one in some fifty.
 
-#include "cache8.cuh"
+#include "cache8_write.cuh"
 
 namespace {
 
 using namespace cache8;
 
 // ------------------------------------------------------------------ write
-struct Write8 {
-    const void *qkv, *wq, *wk;
-    const float *cos_table, *sin_table;
+struct Write8 : Norm8 {
+    const void* qkv;
     const int *tok_pos, *tok_seq, *slots;
     void* q_out;
-    int n_tokens, n_q, n_seqs, table_positions, use_norm, write_kv;
-    float eps;
+    int n_tokens, n_q, n_seqs, write_kv;
 };
-
-// A 64-bit number as 32 bits to be rounded on: what is cut off leaves its mark in the last bit, so that the second rounding is that of the number itself.
-__device__ __forceinline__ float to_be_rounded(double x) {
-    const float f = __double2float_rz(x);
-    return (double)f == x || f != f ? f : __uint_as_float(__float_as_uint(f) | 1u);
-}
-
-// RMSNorm and rotation of a row whose lanes hold N pairs each, pair i of a lane at `at(i)` of the halves; `lanes`: the row's, a power of two of them.
-// Returns whether the position is one of the rotation's.
-template <typename R, int N, typename TW, typename At>
-__device__ __forceinline__ bool norm_rotate(R (&x)[N], R (&y)[N], const Write8& a, const TW* w, int half, int pos, int lanes, unsigned mask, At at) {
-    if (a.use_norm) {
-        R ss = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss += x[i] * x[i] + y[i] * y[i];
-        for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const R inv = (R)1 / sqrt(ss / (R)(2 * half) + (R)a.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (at(i) < half) {
-                x[i] = (x[i] * inv) * (R)to_float(w[at(i)]);
-                y[i] = (y[i] * inv) * (R)to_float(w[at(i) + half]);
-            }
-    }
-    if (a.cos_table) {
-        if ((unsigned)pos >= (unsigned)a.table_positions) return false;
-        const float *cs = a.cos_table + (size_t)pos * half, *sn = a.sin_table + (size_t)pos * half;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (at(i) < half) {
-                const R c = cs[at(i)], s = sn[at(i)], u = x[i], v = y[i];
-                x[i] = u * c - v * s;
-                y[i] = v * c + u * s;
-            }
-    }
-    return true;
-}
 
 // A row's numbers as bytes and the byte of its power; pair i of a lane at `at(i)` of the halves.
 template <int N, typename At>
@@ -146,104 +107,13 @@ __global__ void __launch_bounds__(128) write8_kernel(const GkPages8 p, const Wri
 // queries first, then keys and values), a warp's.  Few tokens: four rows, everything asked for at once (`write8_wide_kernel`).  Many: sixteen, by
 // warps that stay and have the next task's rows and rotation under way in shared memory while they make this one's (`write8_stream_kernel`).  Bound by
 // memory then; through registers the same work is bound by what may be under way in L1, of which the library's shared-memory split leaves 23 KB an SM.
-template <int E, typename T>
-__device__ __forceinline__ void load_run(const T* from, float (&v)[E]);
-template <>
-__device__ __forceinline__ void load_run<4, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[4]) {
-    const uint2 raw = *reinterpret_cast<const uint2*>(from);
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-}
-template <>
-__device__ __forceinline__ void load_run<8, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[8]) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(from);
-    const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __bfloat1622float2(pairs[i]);
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
-}
-template <>
-__device__ __forceinline__ void load_run<4, float>(const float* from, float (&v)[4]) {
-    const float4 f = *reinterpret_cast<const float4*>(from);
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-}
-template <>
-__device__ __forceinline__ void load_run<8, float>(const float* from, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(from + i);
-        v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
-    }
-}
-
-// A key in 64 bits, or a row of values that holds an infinity, by the eight lanes of its row.
-template <int HD, typename TW>
-__device__ __noinline__ void write_row_with_care(const GkPages8& p, const Write8& a, const __nv_bfloat16* row, bool is_v, int pos, long long place, int sub,
-                                                 unsigned mask) {
-    constexpr int E = HD / 16, HALF = HD / 2;
-    const auto at = [&](int i) { return sub * E + i; };
-    float x[E], y[E];
-    load_run<E>(row + sub * E, x);
-    load_run<E>(row + HALF + sub * E, y);
-    if (!is_v) {
-        double u[E], v[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) u[i] = x[i], v[i] = y[i];
-        norm_rotate(u, v, a, (const TW*)a.wk, HALF, pos, 8, mask, at);
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
-    }
-    store_bytes(x, y, (is_v ? p.v : p.k) + place * HD, (is_v ? p.v_exp : p.k_exp) + place, HALF, 8, mask, sub == 0, at);
-}
-
-// Two finite numbers, scaled already, as e4m3: `lo` in the low byte.
-__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-template <int E>
-__device__ __forceinline__ float sum_of_squares(const float (&x)[E], const float (&y)[E]) {  // a tree: seven roundings in a row with the lanes' three
-    float s[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) s[i] = fmaf(x[i], x[i], y[i] * y[i]);
-#pragma unroll
-    for (int n = E / 2; n > 0; n >>= 1)
-#pragma unroll
-        for (int i = 0; i < n; ++i) s[i] += s[i + n];
-    return s[0];
-}
-
-// A row in a lane group's registers to where it belongs: a query (place < 0), a key or a value.
+// A row in a lane group's registers to where it belongs: a query, a key or a value.
 template <int HD, typename TW>
 __device__ __forceinline__ void finish_row(const GkPages8& p, const Write8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16],
                                            const float (&w1)[HD / 16], const float (&c)[HD / 16], const float (&sn)[HD / 16], bool turns, bool is_v,
                                            __nv_bfloat16* q_out, const __nv_bfloat16* in, int pos, long long place, int sub, unsigned mask) {
     constexpr int E = HD / 16, HALF = HD / 2;
-    if (!is_v) {
-        if (a.use_norm) {
-            float ss = sum_of_squares(x, y);
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-            const float inv = rsqrtf(fmaf(ss, 1.f / HD, a.eps));
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                x[i] = (x[i] * inv) * w0[i];
-                y[i] = (y[i] * inv) * w1[i];
-            }
-        }
-        if (turns) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float u = x[i], v = y[i];
-                x[i] = u * c[i] - v * sn[i];
-                y[i] = v * c[i] + u * sn[i];
-            }
-        }
-    }
+    if (!is_v) norm_rotate_32<HD>(a, x, y, w0, w1, c, sn, turns, mask);
     if (q_out) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -258,51 +128,8 @@ __device__ __forceinline__ void finish_row(const GkPages8& p, const Write8& a, f
         }
         return;
     }
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(y[i])));  // (passes over NaN)
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
-    const int b = exponent_byte(top);
-    const float back = power_back(b);
     uint32_t four[2][E / 4];
-    bool care = top == INFINITY;
-    if (is_v || !(a.use_norm || turns)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < E; i += 4)
-                four[h][i / 4] = pack2_finite((h ? y : x)[i] * back, (h ? y : x)[i + 1] * back) | pack2_finite((h ? y : x)[i + 2] * back, (h ? y : x)[i + 3] * back) << 16;
-    } else {
-        // Off by 1.5 * 2^-21 of itself at most through the norm's factor, and by 2^-21 of both numbers that the rotation mixes through the roundings of
-        // their products: where as much less and as much more are not the same byte, or the maximum lies within 2^-18 of the next power's, the row
-        // is made over.
-        care |= abs((int)(__float_as_uint(top) & 0x7fffffu) - 0x600000) < 32;
-        const float slack = 1.25e-6f * back;
-#pragma unroll
-        for (int i = 0; i < E; i += 4) {
-            uint32_t less[2][2], more[2][2];
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                const float t0 = slack * (fabsf(x[i + e]) + fabsf(y[i + e])), t1 = slack * (fabsf(x[i + e + 1]) + fabsf(y[i + e + 1]));
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float u = (h ? y : x)[i + e], v = (h ? y : x)[i + e + 1];
-                    less[h][e / 2] = pack2_finite(fmaf(u, back, -t0), fmaf(v, back, -t1));
-                    more[h][e / 2] = pack2_finite(fmaf(u, back, t0), fmaf(v, back, t1));
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                four[h][i / 4] = less[h][0] | less[h][1] << 16;
-                care |= four[h][i / 4] != (more[h][0] | more[h][1] << 16);
-            }
-        }
-    }
-    if (__any_sync(mask, care)) {
-        write_row_with_care<HD, TW>(p, a, in, is_v, pos, place, sub, mask);
-        return;
-    }
+    const int b = make_bytes<HD, TW>(a, x, y, turns, is_v, in, pos, sub, mask, four);
     uint8_t* to = (is_v ? p.v : p.k) + place * HD + sub * E;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -615,7 +442,7 @@ GK_EXPORT int gk_write8(const GkPages8* pages, const void* qkv, int dtype, const
                table_positions);
     if (n_tokens == 0) return GK_OK;
     GK_REQUIRE(qkv && q_out && tok_pos && tok_seq && slots, "write8: an array is missing");
-    const Write8 a = {qkv, wq, wk, cos_table, sin_table, tok_pos, tok_seq, slots, q_out, n_tokens, n_q, n_seqs, table_positions, use_norm, write_kv, eps};
+    const Write8 a = {{wq, wk, cos_table, sin_table, table_positions, use_norm, eps}, qkv, tok_pos, tok_seq, slots, q_out, n_tokens, n_q, n_seqs, write_kv};
     const long long items = (long long)n_tokens * (n_q + 2 * pages->n_kv), blocks = (items + 3) / 4;
     GK_REQUIRE(blocks < 2147483647LL, "write8: too many tokens");
     if (dtype == GK_BF16 && (pages->head_dim == 64 || pages->head_dim == 128) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)wq | (uintptr_t)wk |

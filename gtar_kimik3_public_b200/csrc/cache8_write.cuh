@@ -1,0 +1,217 @@
+// What is made of a row on its way into the 8-bit cache: RMSNorm and rotation, and its bytes.
+#pragma once
+
+#include "cache8.cuh"
+
+namespace cache8 {
+
+struct Norm8 {
+    const void *wq, *wk;
+    const float *cos_table, *sin_table;  // null: no rotation
+    int table_positions, use_norm;
+    float eps;
+};
+
+// A 64-bit number as 32 bits to be rounded on: what is cut off leaves its mark in the last bit, so that the second rounding is that of the number itself.
+__device__ __forceinline__ float to_be_rounded(double x) {
+    const float f = __double2float_rz(x);
+    return (double)f == x || f != f ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// RMSNorm and rotation of a row whose lanes hold N pairs each, pair i of a lane at `at(i)` of the halves; `lanes`: the row's, a power of two of them.
+// Returns whether the position is one of the rotation's.
+template <typename R, int N, typename TW, typename At>
+__device__ __forceinline__ bool norm_rotate(R (&x)[N], R (&y)[N], const Norm8& a, const TW* w, int half, int pos, int lanes, unsigned mask, At at) {
+    if (a.use_norm) {
+        R ss = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss += x[i] * x[i] + y[i] * y[i];
+        for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const R inv = (R)1 / sqrt(ss / (R)(2 * half) + (R)a.eps);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at(i) < half) {
+                x[i] = (x[i] * inv) * (R)to_float(w[at(i)]);
+                y[i] = (y[i] * inv) * (R)to_float(w[at(i) + half]);
+            }
+    }
+    if (a.cos_table) {
+        if ((unsigned)pos >= (unsigned)a.table_positions) return false;
+        const float *cs = a.cos_table + (size_t)pos * half, *sn = a.sin_table + (size_t)pos * half;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at(i) < half) {
+                const R c = cs[at(i)], s = sn[at(i)], u = x[i], v = y[i];
+                x[i] = u * c - v * s;
+                y[i] = v * c + u * s;
+            }
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------ eight lanes a row of 64 or 128
+template <int E, typename T>
+__device__ __forceinline__ void load_run(const T* from, float (&v)[E]);
+template <>
+__device__ __forceinline__ void load_run<4, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[4]) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(from);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+template <>
+__device__ __forceinline__ void load_run<8, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(from);
+    const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __bfloat1622float2(pairs[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void load_run<4, float>(const float* from, float (&v)[4]) {
+    const float4 f = *reinterpret_cast<const float4*>(from);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+}
+template <>
+__device__ __forceinline__ void load_run<8, float>(const float* from, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(from + i);
+        v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+}
+
+// Two finite numbers, scaled already, as e4m3: `lo` in the low byte.
+__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int E>
+__device__ __forceinline__ float sum_of_squares(const float (&x)[E], const float (&y)[E]) {  // a tree: seven roundings in a row with the lanes' three
+    float s[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[i] = fmaf(x[i], x[i], y[i] * y[i]);
+#pragma unroll
+    for (int n = E / 2; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) s[i] += s[i + n];
+    return s[0];
+}
+
+// The bytes of a key in 64 bits, or of a row of values that holds an infinity, by the eight lanes of its row; the byte of the row's power comes back.
+template <int HD, typename TW>
+__device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, uint32_t* four) {
+    constexpr int E = HD / 16, HALF = HD / 2;
+    const auto at = [&](int i) { return sub * E + i; };
+    float x[E], y[E];
+    load_run<E>(row + sub * E, x);
+    load_run<E>(row + HALF + sub * E, y);
+    if (!is_v) {
+        double u[E], v[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) u[i] = x[i], v[i] = y[i];
+        norm_rotate(u, v, a, (const TW*)a.wk, HALF, pos, 8, mask, at);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+    const int b = exponent_byte(top);
+    const float back = power_back(b);
+    for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < E; i += 4) {
+            const float* z = (h ? y : x) + i;
+            four[h * (E / 4) + i / 4] = pack2(z[0] * back, z[1] * back) | pack2(z[2] * back, z[3] * back) << 16;
+        }
+    return b;
+}
+
+// RMSNorm and rotation of a row in 32 bits.
+template <int HD>
+__device__ __forceinline__ void norm_rotate_32(const Norm8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16], const float (&w1)[HD / 16],
+                                               const float (&c)[HD / 16], const float (&sn)[HD / 16], bool turns, unsigned mask) {
+    constexpr int E = HD / 16;
+    if (a.use_norm) {
+        float ss = sum_of_squares(x, y);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const float inv = rsqrtf(fmaf(ss, 1.f / HD, a.eps));
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] = (x[i] * inv) * w0[i];
+            y[i] = (y[i] * inv) * w1[i];
+        }
+    }
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float u = x[i], v = y[i];
+            x[i] = u * c[i] - v * sn[i];
+            y[i] = v * c[i] + u * sn[i];
+        }
+    }
+}
+
+// A lane's bytes of a key (normed and rotated in 32 bits, `row` what it was made of) or of a row of values; the byte of the row's power comes back.
+template <int HD, typename TW>
+__device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 16], const float (&y)[HD / 16], bool turns, bool is_v, const __nv_bfloat16* row,
+                                          int pos, int sub, unsigned mask, uint32_t (&four)[2][HD / 64]) {
+    constexpr int E = HD / 16;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(y[i])));  // (passes over NaN)
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+    const int b = exponent_byte(top);
+    const float back = power_back(b);
+    bool care = top == INFINITY;
+    if (is_v || !(a.use_norm || turns)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < E; i += 4)
+                four[h][i / 4] = pack2_finite((h ? y : x)[i] * back, (h ? y : x)[i + 1] * back) | pack2_finite((h ? y : x)[i + 2] * back, (h ? y : x)[i + 3] * back) << 16;
+    } else {
+        // Off by 1.5 * 2^-21 of itself at most through the norm's factor, and by 2^-21 of both numbers that the rotation mixes through the roundings of
+        // their products: where as much less and as much more are not the same byte, or the maximum lies within 2^-18 of the next power's, the row
+        // is made over.
+        care |= abs((int)(__float_as_uint(top) & 0x7fffffu) - 0x600000) < 32;
+        const float slack = 1.25e-6f * back;
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+            uint32_t less[2][2], more[2][2];
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float t0 = slack * (fabsf(x[i + e]) + fabsf(y[i + e])), t1 = slack * (fabsf(x[i + e + 1]) + fabsf(y[i + e + 1]));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float u = (h ? y : x)[i + e], v = (h ? y : x)[i + e + 1];
+                    less[h][e / 2] = pack2_finite(fmaf(u, back, -t0), fmaf(v, back, -t1));
+                    more[h][e / 2] = pack2_finite(fmaf(u, back, t0), fmaf(v, back, t1));
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                four[h][i / 4] = less[h][0] | less[h][1] << 16;
+                care |= four[h][i / 4] != (more[h][0] | more[h][1] << 16);
+            }
+        }
+    }
+    if (__any_sync(mask, care)) {
+        uint32_t anew[2 * (E / 4)];
+        const int power = careful_bytes<HD, TW>(a, row, is_v, pos, sub, mask, anew);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) four[h][i] = anew[h * (E / 4) + i];
+        return power;
+    }
+    return b;
+}
+
+}  // namespace cache8

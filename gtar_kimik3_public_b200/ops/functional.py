@@ -2511,20 +2511,9 @@ def _check8(kv: PagedKV8, given: torch.Tensor, *ints: tuple[str, torch.Tensor, i
             raise KernelError(f"{name} must have {entries} entries, got {t.shape[0]}")
 
 
-def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float,
-                        cos: torch.Tensor | None, sin: torch.Tensor | None, tok_pos: torch.Tensor, tok_seq: torch.Tensor, slots: torch.Tensor,
-                        kv: PagedKV8, max_position: int, q_out: torch.Tensor | None = None, write_kv: bool = True) -> torch.Tensor:
-    """``qk_norm_rope_write`` into 8-bit pages: per-head RMSNorm of q and k, rotation by position, and the write of k and v as e4m3 numbers
-    with a power of two a (position, kv head) (see ``PagedKV8``).  Everything is 32-bit up to the one rounding of each result.  Returns the
-    queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
-    _check(qkv, "qkv", dims=2)
-    n = qkv.shape[0]
-    _check8(kv, qkv, ("tok_pos", tok_pos, n), ("tok_seq", tok_seq, n), ("slots", slots, -1))
-    code = dtype_code(qkv.dtype)
-    if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
-        raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
-    if kv._sizes[1] != n_kv or kv._sizes[3] != head_dim:
-        raise KernelError(f"pages {tuple(kv.k.shape)} do not fit n_kv={n_kv}, head_dim={head_dim}")
+def _check_norm8(kv: PagedKV8, q_weight, k_weight, cos, sin) -> tuple[int, int]:
+    """The type of the norm weights and the positions of the rotation's tables."""
+    head_dim, index = kv._sizes[3], kv._index
     weight_code = table_positions = 0
     if (q_weight is None) != (k_weight is None):
         raise KernelError("q and k are normed both or neither")
@@ -2542,6 +2531,27 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
         if cos.shape[1] != head_dim // 2 or sin.shape != cos.shape:
             raise KernelError("rotary tables must be [positions, head_dim / 2]")
         table_positions = cos.shape[0]
+    for name, t in (("norm weights", q_weight), ("norm weights", k_weight), ("rotary tables", cos), ("rotary tables", sin)):
+        if t is not None and t.get_device() != index:
+            raise KernelError(f"{name} are on {t.device}, the pages on {kv.k.device}")
+    return weight_code, table_positions
+
+
+def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float,
+                        cos: torch.Tensor | None, sin: torch.Tensor | None, tok_pos: torch.Tensor, tok_seq: torch.Tensor, slots: torch.Tensor,
+                        kv: PagedKV8, max_position: int, q_out: torch.Tensor | None = None, write_kv: bool = True) -> torch.Tensor:
+    """``qk_norm_rope_write`` into 8-bit pages: per-head RMSNorm of q and k, rotation by position, and the write of k and v as e4m3 numbers
+    with a power of two a (position, kv head) (see ``PagedKV8``).  Everything is 32-bit up to the one rounding of each result.  Returns the
+    queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
+    _check(qkv, "qkv", dims=2)
+    n = qkv.shape[0]
+    _check8(kv, qkv, ("tok_pos", tok_pos, n), ("tok_seq", tok_seq, n), ("slots", slots, -1))
+    code = dtype_code(qkv.dtype)
+    if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
+        raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
+    if kv._sizes[1] != n_kv or kv._sizes[3] != head_dim:
+        raise KernelError(f"pages {tuple(kv.k.shape)} do not fit n_kv={n_kv}, head_dim={head_dim}")
+    weight_code, table_positions = _check_norm8(kv, q_weight, k_weight, cos, sin)
     if q_out is None:
         q_out = torch.empty((n, n_q, head_dim), dtype=qkv.dtype, device=qkv.device)
     else:
@@ -2627,21 +2637,56 @@ def rows8_cut(pairs: int, kv_len: int, places: tuple[int, int, int, int]) -> tup
     return 1 << best, 0
 
 
+def _cut8(kv: PagedKV8, n_rows: int, n_tiles: int, kv_len_hint: int, cut: tuple[int, int] | None) -> tuple[int, int, int, torch.Tensor | None]:
+    """Rows taken together, splits, pieces and scratch of a call over ``n_tiles`` times ``n_rows`` rows a kv head."""
+    _, n_kv, _, d = kv._sizes
+    rows = 8 if n_rows <= 8 else 16
+    pairs = n_tiles * -(-n_rows // rows) * n_kv
+    splits, pieces = rows8_cut(pairs, kv_len_hint, rows8_places(d, rows, _sm_count_of(kv._index))) if cut is None else cut
+    scratch = None
+    if splits == 0:
+        scratch = torch.empty(((pieces + pairs) * rows * (d + 3),), dtype=torch.float32, device=kv.k.device)
+    return rows, splits, pieces, scratch
+
+
 def _rows8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor | None, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, kv_len_hint: int,
            scale: float, window: int, sink: bool, cut: tuple[int, int] | None, out: torch.Tensor) -> torch.Tensor:
     n_seqs, n_q = kv_len.shape[0], q.shape[1]
-    _, n_kv, _, d = kv._sizes
-    n_rows = max_q_len * (n_q // n_kv)
-    rows = 8 if n_rows <= 8 else 16
-    pairs = n_seqs * -(-n_rows // rows) * n_kv
-    if cut is None:
-        cut = rows8_cut(pairs, min(kv_len_hint, window + max_q_len) if window else kv_len_hint, rows8_places(d, rows, _sm_count_of(kv._index)))
-    splits, pieces = cut
-    scratch = None
-    if splits == 0:
-        scratch = torch.empty(((pieces + pairs) * rows * (d + 3),), dtype=torch.float32, device=q.device)
+    hint = min(kv_len_hint, window + max_q_len) if window else kv_len_hint
+    rows, splits, pieces, scratch = _cut8(kv, max_q_len * (n_q // kv._sizes[1]), n_seqs, hint, cut)
     call("gk_rows8", kv._at, ptr(q), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), n_seqs, n_q, max_q_len, rows, splits, pieces, ptr(scratch),
          float(scale), int(window), int(sink), stream_ptr())
+    return out
+
+
+def decode8_fused_ok(qkv: torch.Tensor, kv: PagedKV8, n_q: int) -> bool:
+    """Whether the decode kernel that also norms, rotates and writes the new token takes the layer."""
+    _, n_kv, page, d = kv._sizes
+    return qkv.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and n_q // n_kv <= ROWS8_MAX_GROUP
+
+
+def attention_decode8_fused(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                            eps: float, cos: torch.Tensor | None, sin: torch.Tensor | None, kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor,
+                            max_position: int, max_kv_len: int, scale: float, window: int = 0, write_kv: bool = True,
+                            cut: tuple[int, int] | None = None) -> torch.Tensor:
+    """``qk_norm_rope_write8`` and ``attention_decode8`` of one new token per sequence in one kernel, from the packed projection
+    ``qkv [n_seqs, (n_q + 2 n_kv) * head_dim]`` (bfloat16, heads of 64 or 128, pages of 64).  The cache gets the same bytes; the queries are not
+    rounded to bfloat16 on the way.  Returns ``[n_seqs, n_q, head_dim]``."""
+    _check(qkv, "qkv", torch.bfloat16, 2)
+    n = qkv.shape[0]
+    _check8(kv, qkv, ("kv_len", kv_len, n), ("slots", slots, n))
+    if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
+        raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
+    if kv._sizes[1] != n_kv or kv._sizes[3] != head_dim or n_q % n_kv:
+        raise KernelError(f"pages {tuple(kv.k.shape)} do not fit n_q={n_q}, n_kv={n_kv}, head_dim={head_dim}")
+    if not decode8_fused_ok(qkv, kv, n_q):
+        raise KernelError(f"one kernel takes heads of {ROWS8_HEAD_DIMS}, pages of 64 and up to {ROWS8_MAX_GROUP} query heads a kv head")
+    weight_code, table_positions = _check_norm8(kv, q_weight, k_weight, cos, sin)
+    out = torch.empty((n, n_q, head_dim), dtype=torch.bfloat16, device=qkv.device)
+    rows, splits, pieces, scratch = _cut8(kv, n_q // n_kv, n, min(max_kv_len, window + 1) if window else max_kv_len, cut)
+    call("gk_rows8_fused", kv._at, ptr(qkv), ptr(q_weight), ptr(k_weight), weight_code, int(q_weight is not None), float(eps), ptr(cos), ptr(sin),
+         table_positions, int(max_position), int(write_kv), ptr(out), ptr(kv_len), ptr(slots), n, n_q, rows, splits, pieces, ptr(scratch), float(scale),
+         int(window), stream_ptr())
     return out
 
 

@@ -267,6 +267,45 @@ def test_decode(dtype, cut, n_q, n_kv, d, window, sink):
     F().check_kernel_errors(DEV)
 
 
+@pytest.mark.parametrize("n_q,n_kv,d", [(16, 8, 128), (8, 1, 128), (12, 1, 128), (16, 1, 64), (6, 2, 64), (1, 1, 64)])
+@pytest.mark.parametrize("cut", [None, (1, 0), (4, 0), (0, 1), (0, 40)])
+@pytest.mark.parametrize("window,norm,weights", [(0, True, torch.float32), (70, True, torch.bfloat16), (0, False, torch.float32)])
+def test_decode_from_the_projection(n_q, n_kv, d, cut, window, norm, weights):
+    """Norm, rotation, write and attention in one kernel: the cache gets the bytes that the write gives, the places around them stay, and the
+    outputs are those of attention over them."""
+    lens, eps = [1, 64, 65, 300, 777, 97, 32, 33], 1e-5
+    n = len(lens)
+    kv, slots, table = empty_pages(n, max(lens), n_kv, d)
+    for i, m in enumerate(lens):  # all but the new token
+        k, v = rand(m - 1, n_kv, d, seed=30 + i), rand(m - 1, n_kv, d, seed=60 + i)
+        fill(kv, table, int(slots[i]), k, v, max(0, m - window) if window else 0)
+    copy = F().PagedKV8(kv.k.view(torch.uint8).clone().view(torch.float8_e4m3fn), kv.v.view(torch.uint8).clone().view(torch.float8_e4m3fn),
+                        kv.k_exp.clone(), kv.v_exp.clone(), kv.block_table)
+    qkv = rand(n, (n_q + 2 * n_kv) * d, seed=7).to(torch.bfloat16)
+    qkv[3, n_q * d:] = 0
+    wq, wk = (1 + 0.1 * rand(d, seed=20)).to(weights).to(DEV), (1 + 0.1 * rand(d, seed=21)).to(weights).to(DEV)
+    cos, sin = plain.rotary_tables(torch.arange(max(lens)), d, 1e4)
+    cos, sin = cos[:, : d // 2].float().contiguous().to(DEV), sin[:, : d // 2].float().contiguous().to(DEV)
+    how = (wq, wk, eps, cos, sin) if norm else (None, None, eps, None, None)
+    pos = ints(*[m - 1 for m in lens])
+    F().qk_norm_rope_write8(qkv.to(DEV), n_q, n_kv, d, *how, pos, ints(*range(n)), slots, copy, max(lens) - 1)
+    got = F().attention_decode8_fused(qkv.to(DEV), n_q, n_kv, d, *how, kv, ints(*lens), slots, max(lens) - 1, 777, d**-0.5, window, cut=cut)
+    F().check_kernel_errors(DEV)
+    for a, b in ((kv.k, copy.k), (kv.v, copy.v), (kv.k_exp, copy.k_exp), (kv.v_exp, copy.v_exp)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    x = qkv.double().view(n, n_q + 2 * n_kv, d)[:, :n_q]
+    if norm:
+        c, s = (torch.cat([t, t], -1).double().cpu()[[m - 1 for m in lens]] for t in (cos, sin))
+        x = plain.apply_rotary(plain.rms_norm(x, wq.double().cpu(), eps), c, s)
+    for i, m in enumerate(lens):
+        k, v = held(kv, table, int(slots[i]), m)
+        # queries in 32 bits: 2^-20 of scores of up to some twenty
+        check_attention(got[i:i + 1], x[i:i + 1], k, v, m - 1, window, False, SINGLE[torch.bfloat16] + 2.0**-15, f"sequence of {m}")
+    # a layer that attends over what another has written
+    again = F().attention_decode8_fused(qkv.to(DEV), n_q, n_kv, d, *how, kv, ints(*lens), slots, max(lens) - 1, 777, d**-0.5, window, write_kv=False, cut=cut)
+    assert torch.equal(again, got)
+
+
 @pytest.mark.parametrize("dtype,few", [(torch.bfloat16, None), (torch.bfloat16, True), (torch.bfloat16, False), (torch.float32, None)])
 @pytest.mark.parametrize("n_q,n_kv,d", GROUPS)
 @pytest.mark.parametrize("window,sink", [(0, False), (70, True)])
