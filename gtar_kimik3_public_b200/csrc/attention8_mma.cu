@@ -269,47 +269,40 @@ __device__ __forceinline__ void norm_rotate_queries(const Fused8& f, float (&x)[
     }
 }
 
-// The new key and value of a sequence: lanes 0 .. 7 the key, 8 .. 15 the value.
+// The new key and value of a sequence, a warp's work, D / 64 numbers of each half a lane.  Always the careful way: two numbers a lane take less long than
+// code that is run for one key in fifty takes to be fetched (one kernel of 64 such keys: 3 us).
 template <int D, typename TW>
 __device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, const Fused8& f, const Unit& u, int hk, int lane, unsigned char (&bytes)[2][D],
                                          unsigned char (&powers)[2]) {
-    constexpr int E = D / 16, HALF = D / 2;
-    const int sub = lane & 7, pos = u.past;
-    const bool is_v = lane >= 8;
-    const unsigned mask = 0xffu << (lane & 24);
-    if (lane < 16) {
-        const __nv_bfloat16* row = f.qkv + ((size_t)u.first_token * (a.n_q + 2 * p.n_kv) + a.n_q + (is_v ? p.n_kv : 0) + hk) * D;
-        float x[E], y[E], w0[E], w1[E], c[E], sn[E];
-        load_run<E>(row + sub * E, x);
-        load_run<E>(row + HALF + sub * E, y);
-        const bool turns = f.cos_table != nullptr && !is_v && (unsigned)pos < (unsigned)f.table_positions;
-        if (f.cos_table != nullptr && (unsigned)pos >= (unsigned)f.table_positions && p.error) *p.error = ERR_PLACE;
-        if (!is_v) {
-            if (f.use_norm) {
-                load_run<E>((const TW*)f.wk + sub * E, w0);
-                load_run<E>((const TW*)f.wk + HALF + sub * E, w1);
+    constexpr int E = D / 64, HALF = D / 2;
+    const int pos = u.past;
+    const __nv_bfloat16* row = f.qkv + ((size_t)u.first_token * (a.n_q + 2 * p.n_kv) + a.n_q + hk) * D;
+    if (f.cos_table != nullptr && (unsigned)pos >= (unsigned)f.table_positions && p.error) *p.error = ERR_PLACE;
+    float x[2][2][E];
+    int b[2];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) b[v] = careful_row<D, 32, TW>(f, row + (size_t)v * p.n_kv * D, v == 1, pos, lane, 0xffffffffu, x[v]);
+    const int page = page_of(p, u.slot, pos / PAGE);
+    const size_t place = ((size_t)max(page, 0) * p.n_kv + hk) * PAGE + pos % PAGE;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const float back = power_back(b[v]);
+        uint8_t* to = (v ? p.v : p.k) + place * D;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = h * HALF + lane * E;
+            const uint32_t two = pack2(x[v][h][0] * back, x[v][h][E - 1] * back);
+            if constexpr (E == 2) {
+                *reinterpret_cast<uint16_t*>(&bytes[v][at]) = (uint16_t)two;
+                if (page >= 0) *reinterpret_cast<uint16_t*>(to + at) = (uint16_t)two;
+            } else {
+                bytes[v][at] = (unsigned char)two;
+                if (page >= 0) to[at] = (uint8_t)two;
             }
-            if (turns) {
-                load_run<E>(f.cos_table + (size_t)pos * HALF + sub * E, c);
-                load_run<E>(f.sin_table + (size_t)pos * HALF + sub * E, sn);
-            }
-            norm_rotate_32<D>(f, x, y, w0, w1, c, sn, turns, mask);
         }
-        uint32_t four[2][E / 4];
-        const int b = make_bytes<D, TW>(f, x, y, turns, is_v, row, pos, sub, mask, four);
-        const int page = page_of(p, u.slot, pos / PAGE);
-        const size_t place = ((size_t)max(page, 0) * p.n_kv + hk) * PAGE + pos % PAGE;
-        uint8_t* to = (is_v ? p.v : p.k) + place * D + sub * E;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < E / 4; ++i) {
-                *reinterpret_cast<uint32_t*>(&bytes[is_v][h * HALF + sub * E + 4 * i]) = four[h][i];
-                if (page >= 0) *reinterpret_cast<uint32_t*>(to + h * HALF + 4 * i) = four[h][i];
-            }
-        if (sub == 0) {
-            powers[is_v] = (unsigned char)b;
-            if (page >= 0) (is_v ? p.v_exp : p.k_exp)[place] = (uint8_t)b;
+        if (lane == 0) {
+            powers[v] = (unsigned char)b[v];
+            if (page >= 0) (v ? p.v_exp : p.k_exp)[place] = (uint8_t)b[v];
         }
     }
     __syncwarp();

@@ -2,10 +2,10 @@
 //
 // The write does the attention input stage too, as the 16-bit cache's does: per-head RMSNorm of q and k (src/layers/rmsnorm.py:11-16),
 // rotation (src/layers/rope.py:17-33), order of src/layers/attention.py:82-89.  Queries are 32-bit up to the one rounding to their type, values are only
-// rounded.  Keys come out as the formula in 64 bits rounded once: e4m3's steps are so coarse that a number 2^-22 beside the middle between two of
-// them goes wrong by a sixteenth of itself, which 32 bits do to some three in a million.  All of it in 64 bits is slow (7,921 tokens of 32/8 heads of
-// 128: 50 us more), so the wide kernel makes them in 32 bits and does over, in 64, the rows that have a number or their maximum next to a border:
-// one in some fifty.
+// rounded.  Keys come out as the formula in 64 bits (or, in the wide kernels, some 45) rounded once: e4m3's steps are so coarse that a number 2^-22 beside the
+// middle between two of them goes wrong by a sixteenth of itself, which 32 bits do to some three in a million.  The wide kernels make a key in 32
+// bits and do it over where a number or its maximum lies next to a border, one row in some fifty (7,921 tokens of 32/8 heads of 128: 49 us; with
+// every key in 64 bits 127).
 
 #include "cache8_write.cuh"
 

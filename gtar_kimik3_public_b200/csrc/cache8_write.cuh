@@ -82,6 +82,21 @@ __device__ __forceinline__ void load_run<8, float>(const float* from, float (&v)
     }
 }
 
+template <>
+__device__ __forceinline__ void load_run<2, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[2]) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(from));
+    v[0] = f.x, v[1] = f.y;
+}
+template <>
+__device__ __forceinline__ void load_run<1, __nv_bfloat16>(const __nv_bfloat16* from, float (&v)[1]) { v[0] = __bfloat162float(*from); }
+template <>
+__device__ __forceinline__ void load_run<2, float>(const float* from, float (&v)[2]) {
+    const float2 f = *reinterpret_cast<const float2*>(from);
+    v[0] = f.x, v[1] = f.y;
+}
+template <>
+__device__ __forceinline__ void load_run<1, float>(const float* from, float (&v)[1]) { v[0] = *from; }
+
 // Two finite numbers, scaled already, as e4m3: `lo` in the low byte.
 __device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
     uint16_t r;
@@ -101,33 +116,116 @@ __device__ __forceinline__ float sum_of_squares(const float (&x)[E], const float
     return s[0];
 }
 
-// The bytes of a key in 64 bits, or of a row of values that holds an infinity, by the eight lanes of its row; the byte of the row's power comes back.
-template <int HD, typename TW>
-__device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, uint32_t* four) {
-    constexpr int E = HD / 16, HALF = HD / 2;
-    const auto at = [&](int i) { return sub * E + i; };
-    float x[E], y[E];
-    load_run<E>(row + sub * E, x);
-    load_run<E>(row + HALF + sub * E, y);
+// ------------------------------------------------------------------ a key as the formula in some 45 bits, rounded once
+// A number as the sum of two 32-bit ones, the second at most half a step of the first: sums and products of two numbers are exact as such pairs (Dekker;
+// Knuth).  64-bit arithmetic is a sixteenth as fast here.
+struct Two8 {
+    float h, l;
+};
+__device__ __forceinline__ Two8 sum_of(float a, float b) {
+    const float s = __fadd_rn(a, b), t = __fsub_rn(s, a);
+    return {s, __fadd_rn(__fsub_rn(a, __fsub_rn(s, t)), __fsub_rn(b, t))};
+}
+__device__ __forceinline__ Two8 product_of(float a, float b) {
+    const float p = __fmul_rn(a, b);
+    return {p, __fmaf_rn(a, b, -p)};
+}
+// The pair as 32 bits to be rounded on: what is cut off leaves its mark in the last bit.
+__device__ __forceinline__ float to_be_rounded(float high, float low) {
+    const float h = __fadd_rn(high, low), l = __fsub_rn(low, __fsub_rn(h, high));
+    if (!(fabsf(h) < INFINITY) || l == 0.f) return fabsf(high) < INFINITY ? h : high;
+    return __uint_as_float((__float_as_uint(h) - ((l < 0.f) != (h < 0.f) ? 1u : 0u)) | 1u);
+}
+
+// A key, or a row of values as it is, by LANES lanes that have HD / 2 / LANES neighbouring numbers of each half: the numbers to be rounded; the byte of the
+// row's power comes back.
+template <int HD, int LANES, typename TW>
+__device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, float (&x)[2][HD / 2 / LANES]) {
+    constexpr int E = HD / 2 / LANES, HALF = HD / 2;
+    float low[2][E];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        load_run<E>(row + h * HALF + sub * E, x[h]);
+#pragma unroll
+        for (int i = 0; i < E; ++i) low[h][i] = 0.f;
+    }
     if (!is_v) {
-        double u[E], v[E];
+        if (a.use_norm) {
+            Two8 ss = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < E; ++i) u[i] = x[i], v[i] = y[i];
-        norm_rotate(u, v, a, (const TW*)a.wk, HALF, pos, 8, mask, at);
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = to_be_rounded(u[i]), y[i] = to_be_rounded(v[i]);
+                for (int i = 0; i < E; ++i) {  // (the square of a bfloat16 number is exact)
+                    const Two8 t = sum_of(ss.h, __fmul_rn(x[h][i], x[h][i]));
+                    ss = {t.h, __fadd_rn(ss.l, t.l)};
+                }
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) {
+                const float oh = __shfl_xor_sync(mask, ss.h, o), ol = __shfl_xor_sync(mask, ss.l, o);
+                const Two8 t = sum_of(ss.h, oh);
+                ss = {t.h, __fadd_rn(t.l, __fadd_rn(ss.l, ol))};
+            }
+            const Two8 m = sum_of(ss.h * (1.f / HD), a.eps);  // (HD is a power of two)
+            const float ml = fmaf(ss.l, 1.f / HD, m.l);
+            float r = rsqrtf(m.h), dr = 0.f;
+            if (m.h < INFINITY && m.h > 0.f) {  // 1 / sqrt(m) = r + dr: a step of Newton's
+                const Two8 rr = product_of(r, r);
+                const float e = __fsub_rn(__fmaf_rn(-rr.h, m.h, 1.f), __fmaf_rn(rr.l, m.h, __fmul_rn(rr.h, ml)));
+                dr = 0.5f * r * e;
+            }
+            float w[2][E];
+            load_run<E>((const TW*)a.wk + sub * E, w[0]);
+            load_run<E>((const TW*)a.wk + HALF + sub * E, w[1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const Two8 p = product_of(x[h][i], w[h][i]), z = product_of(p.h, r);
+                    x[h][i] = z.h;
+                    low[h][i] = __fadd_rn(z.l, __fmaf_rn(p.h, dr, __fmul_rn(p.l, r)));
+                }
+        }
+        if (a.cos_table && (unsigned)pos < (unsigned)a.table_positions) {
+            float c[E], sn[E];
+            load_run<E>(a.cos_table + (size_t)pos * HALF + sub * E, c);
+            load_run<E>(a.sin_table + (size_t)pos * HALF + sub * E, sn);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float u = x[0][i], v = x[1][i], ul = low[0][i], vl = low[1][i];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float s = h ? sn[i] : -sn[i];
+                    const Two8 p = product_of(h ? v : u, c[i]), q = product_of(h ? u : v, s), t = sum_of(p.h, q.h);
+                    x[h][i] = t.h;
+                    low[h][i] = __fadd_rn(__fadd_rn(t.l, __fadd_rn(p.l, q.l)), __fmaf_rn(h ? vl : ul, c[i], __fmul_rn(h ? ul : vl, s)));
+                }
+            }
+        }
     }
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = fmaxf(top, fmaxf(finite_abs(x[i]), finite_abs(y[i])));
-    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
-    const int b = exponent_byte(top);
-    const float back = power_back(b);
     for (int h = 0; h < 2; ++h)
-        for (int i = 0; i < E; i += 4) {
-            const float* z = (h ? y : x) + i;
-            four[h * (E / 4) + i / 4] = pack2(z[0] * back, z[1] * back) | pack2(z[2] * back, z[3] * back) << 16;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[h][i] = to_be_rounded(x[h][i], low[h][i]);
+            top = fmaxf(top, finite_abs(x[h][i]));
         }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+    return exponent_byte(top);
+}
+// The same by eight lanes, as bytes.
+template <int HD, typename TW>
+__device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, uint32_t* four) {
+    constexpr int E = HD / 16;
+    float x[2][E];
+    const int b = careful_row<HD, 8, TW>(a, row, is_v, pos, sub, mask, x);
+    const float back = power_back(b);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+            four[h * (E / 4) + i / 4] = pack2(x[h][i] * back, x[h][i + 1] * back) | pack2(x[h][i + 2] * back, x[h][i + 3] * back) << 16;
     return b;
 }
 
@@ -169,7 +267,8 @@ __device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 
     for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
     const int b = exponent_byte(top);
     const float back = power_back(b);
-    bool care = top == INFINITY;
+    // (a row that holds an infinity or NaN and is normed: its maximum is 0 or not to be trusted)
+    bool care = top == INFINITY || (!is_v && a.use_norm && top == 0.f);
     if (is_v || !(a.use_norm || turns)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
