@@ -29,7 +29,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from ..ops.functional import DecodeWork, PagedKV, PagedKV8, PagedRows, Work8
+from ..ops.functional import DecodeWork, PagedKV, PagedKV8, PagedRows
 from ..parts.base import KVRequest, RowsRequest, StateRequest
 from .allocators import CacheFull, PageAllocator, SlotAllocator
 
@@ -87,7 +87,7 @@ class _KVGroup:
         self.upto: dict[int, int] = {}  # slot -> one past the highest page index the sequence ever had
         self.dirty: set[int] = set()
         self._staging = None  # pinned copies of the table for uploads, made at the first upload
-        self._work = None  # attention's scratch for this group's layers, made with the first view
+        self._work = None  # decode attention's scratch for this group's layers, made with the first view
         self._views: dict[tuple[int, int], PagedKV8] = {}
 
     def open_slot(self, slot: int) -> None:
@@ -170,9 +170,7 @@ class _KVGroup:
         i = self.index_of[item]
         if isinstance(self.request, KVRequest) and self.request.dtype is not None:
             if item not in self._views:
-                if self._work is None:
-                    self._work = Work8(self.table.device)
-                self._views[item] = PagedKV8(self.k[i], self.v[i], self.k_exp[i], self.v_exp[i], self.table, self._work)
+                self._views[item] = PagedKV8(self.k[i], self.v[i], self.k_exp[i], self.v_exp[i], self.table)
             return self._views[item]
         if self.v is None:
             return PagedRows(self.k[i], self.table)
@@ -315,6 +313,11 @@ class Cache:
             else:
                 total += len(group.items) * r.n_kv_heads * (r.head_dim + (r.value_dim or r.head_dim)) * self.k_element_size()
         return total
+
+    def scratch_bytes_per_token(self) -> int:
+        """What a step may need for a moment besides the cache, for each token that it holds: prompts attend over one layer's 8-bit pages at a time
+        made bfloat16."""
+        return max([4 * g.request.n_kv_heads * g.request.head_dim for g in self.kv_groups if getattr(g.request, "dtype", None) is not None], default=0)
 
     def k_element_size(self) -> int:
         return torch.empty((), dtype=self.dtype).element_size()

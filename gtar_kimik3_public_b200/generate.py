@@ -74,7 +74,8 @@ class Generator:
         configuration may allow tens of thousands of positions, far more than a batch of them fits)."""
         longest = getattr(model.config, "max_position_embeddings", None) or 4096
         wanted = max_batch * rounded_tokens(longest)
-        per_token = model.make_cache(rounded_tokens(1), 1).kv_bytes_per_token()
+        small = model.make_cache(rounded_tokens(1), 1)
+        per_token = small.kv_bytes_per_token() + small.scratch_bytes_per_token()
         if model.device.type != "cuda" or per_token == 0:
             return wanted
         free, _ = torch.cuda.mem_get_info(model.device)

@@ -2454,7 +2454,6 @@ class PagedKV8:
     k_exp: torch.Tensor
     v_exp: torch.Tensor
     block_table: torch.Tensor
-    work: "Work8 | None" = None  # what attention keeps between launches; the cache group owns it
 
     def __post_init__(self):
         require_device(self.k.device)
@@ -2471,8 +2470,6 @@ class PagedKV8:
             raise KernelError(f"exponents must be {tuple(self.k.shape[:3])}, got {tuple(self.k_exp.shape)} and {tuple(self.v_exp.shape)}")
         if page % 32 or d % 2 or not 0 < d <= CACHE8_MAX_HEAD_DIM:
             raise KernelError(f"8-bit pages take a page size that is a multiple of 32 and an even head size up to {CACHE8_MAX_HEAD_DIM}, got {page} and {d}")
-        if self.work is None:
-            object.__setattr__(self, "work", Work8(self.k.device))
         pages = _Pages8(ptr(self.k), ptr(self.v), ptr(self.k_exp), ptr(self.v_exp), ptr(self.block_table), ptr(error_flag(self.k.device)), n_pages,
                         self.block_table.shape[0], self.block_table.shape[1], n_kv, page, d)
         object.__setattr__(self, "_pages", pages)
@@ -2487,13 +2484,6 @@ class PagedKV8:
     @property
     def max_pages(self) -> int:
         return self.block_table.shape[1]
-
-
-class Work8:
-    """Memory that attention over 8-bit pages keeps between launches, one per cache group (its layers run one after another on one stream)."""
-
-    def __init__(self, device: torch.device):
-        self.device = device
 
 
 def _check8(kv: PagedKV8, given: torch.Tensor, *ints: tuple[str, torch.Tensor, int]) -> None:
