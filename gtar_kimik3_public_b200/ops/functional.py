@@ -2475,7 +2475,7 @@ class PagedKV8:
         object.__setattr__(self, "_pages", pages)
         object.__setattr__(self, "_at", ctypes.addressof(pages))
         object.__setattr__(self, "_index", self.k.get_device())
-        object.__setattr__(self, "_sizes", (n_pages, n_kv, page, d))
+        object.__setattr__(self, "_sizes", (n_pages, n_kv, page, d))  # plain numbers
 
     @property
     def page_size(self) -> int:
@@ -2486,9 +2486,18 @@ class PagedKV8:
         return self.block_table.shape[1]
 
 
+_INT32, _BFLOAT16 = torch.int32, torch.bfloat16
+
+
+def _fine8(kv: PagedKV8, given: torch.Tensor, a: torch.Tensor, b: torch.Tensor, shape: tuple) -> bool:
+    """Whether ``_check8`` has nothing to say of two int32 vectors of this shape, in one expression: a call of few microseconds is asked for in as many."""
+    index = kv._index
+    return (a.dtype is _INT32 and b.dtype is _INT32 and a.shape == shape and b.shape == shape and a.is_contiguous() and b.is_contiguous()
+            and given.get_device() == index and a.get_device() == index and b.get_device() == index and current_device() == index)
+
+
 def _check8(kv: PagedKV8, given: torch.Tensor, *ints: tuple[str, torch.Tensor, int]) -> None:
-    """What every call over 8-bit pages asks of its tensors: ``ints`` are (name, int32 tensor, entries or -1).  (Device numbers and not
-    ``torch.device``: a call of few microseconds is asked for in as many.)"""
+    """What every call over 8-bit pages asks of its tensors: ``ints`` are (name, int32 tensor, entries or -1)."""
     index = kv._index
     if given.get_device() != index:
         raise KernelError(f"the tensors are on {given.device}, the pages on {kv.k.device}")
@@ -2504,6 +2513,11 @@ def _check8(kv: PagedKV8, given: torch.Tensor, *ints: tuple[str, torch.Tensor, i
 def _check_norm8(kv: PagedKV8, q_weight, k_weight, cos, sin) -> tuple[int, int]:
     """The type of the norm weights and the positions of the rotation's tables."""
     head_dim, index = kv._sizes[3], kv._index
+    if (q_weight is not None and k_weight is not None and cos is not None and sin is not None and q_weight.dtype is k_weight.dtype
+            and q_weight.shape == k_weight.shape == (head_dim,) and cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] * 2 == head_dim
+            and cos.dtype is torch.float32 and sin.dtype is torch.float32 and q_weight.is_contiguous() and k_weight.is_contiguous() and cos.is_contiguous()
+            and sin.is_contiguous() and q_weight.get_device() == k_weight.get_device() == cos.get_device() == sin.get_device() == index):
+        return dtype_code(q_weight.dtype), cos.shape[0]  # the usual layer, in one expression
     weight_code = table_positions = 0
     if (q_weight is None) != (k_weight is None):
         raise KernelError("q and k are normed both or neither")
@@ -2531,14 +2545,15 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
                         cos: torch.Tensor | None, sin: torch.Tensor | None, tok_pos: torch.Tensor, tok_seq: torch.Tensor, slots: torch.Tensor,
                         kv: PagedKV8, max_position: int, q_out: torch.Tensor | None = None, write_kv: bool = True) -> torch.Tensor:
     """``qk_norm_rope_write`` into 8-bit pages: per-head RMSNorm of q and k, rotation by position, and the write of k and v as e4m3 numbers
-    with a power of two a (position, kv head) (see ``PagedKV8``).  Everything is 32-bit up to the one rounding of each result.  Returns the
-    queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
+    with a power of two a (position, kv head) (see ``PagedKV8``).  Queries are 32-bit up to their one rounding; keys and values are kept as the
+    formula in 64 bits rounded once.  Returns the queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
     _check(qkv, "qkv", dims=2)
-    n = qkv.shape[0]
-    _check8(kv, qkv, ("tok_pos", tok_pos, n), ("tok_seq", tok_seq, n), ("slots", slots, -1))
+    n, width = qkv.shape
+    if not (_fine8(kv, qkv, tok_pos, tok_seq, (n,)) and _fine8(kv, qkv, slots, slots, slots.shape) and slots.dim() == 1):
+        _check8(kv, qkv, ("tok_pos", tok_pos, n), ("tok_seq", tok_seq, n), ("slots", slots, -1))
     code = dtype_code(qkv.dtype)
-    if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
-        raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
+    if width != (n_q + 2 * n_kv) * head_dim:
+        raise KernelError(f"qkv rows are {width} wide, expected {(n_q + 2 * n_kv) * head_dim}")
     if kv._sizes[1] != n_kv or kv._sizes[3] != head_dim:
         raise KernelError(f"pages {tuple(kv.k.shape)} do not fit n_kv={n_kv}, head_dim={head_dim}")
     weight_code, table_positions = _check_norm8(kv, q_weight, k_weight, cos, sin)
@@ -2548,25 +2563,26 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
         _check(q_out, "q_out", qkv.dtype, 3)
         if q_out.shape != (n, n_q, head_dim):
             raise KernelError(f"q_out is {tuple(q_out.shape)}, expected {(n, n_q, head_dim)}")
-    call("gk_write8", kv._at, ptr(qkv), code, ptr(q_weight), ptr(k_weight), weight_code, int(q_weight is not None), float(eps), ptr(cos), ptr(sin),
-         table_positions, int(max_position), ptr(tok_pos), ptr(tok_seq), ptr(slots), slots.shape[0], ptr(q_out), n, n_q, int(write_kv), stream_ptr())
+    call("gk_write8", kv._at, qkv.data_ptr(), code, ptr(q_weight), ptr(k_weight), weight_code, q_weight is not None, float(eps), ptr(cos), ptr(sin),
+         table_positions, int(max_position), tok_pos.data_ptr(), tok_seq.data_ptr(), slots.data_ptr(), slots.shape[0], q_out.data_ptr(), n, n_q, bool(write_kv),
+         stream_ptr())
     return q_out
 
 
 def read_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, out: PagedKV | None = None, last: int = 0) -> PagedKV:
     """The 8-bit pages of the listed sequences read back, exactly, as bfloat16 pages of the same numbers: those that hold each sequence's last
     ``last`` positions (0: all).  Places behind a sequence's end in its last page become zero; pages that the step does not name are left as they
-    were.  ``out``: pages of the same shape (made here if there are none); ``max_kv_len``: the longest of ``kv_len``, known on the host."""
+    were (in pages made here, ``out`` None: undefined).  ``out``: pages of the same shape; ``max_kv_len``: the longest of ``kv_len``, known on the host."""
     n = kv_len.shape[0]
-    _check8(kv, kv_len, ("kv_len", kv_len, n), ("slots", slots, n))
+    if not _fine8(kv, kv_len, kv_len, slots, (n,)):
+        _check8(kv, kv_len, ("kv_len", kv_len, n), ("slots", slots, n))
     if out is None:
         k, v = (torch.empty(kv.k.shape, dtype=torch.bfloat16, device=kv.k.device) for _ in range(2))
         out = PagedKV(k, v, kv.block_table)
     for name, t in (("k pages", out.k), ("v pages", out.v)):
-        _check(t, name, torch.bfloat16, 4)
-        if t.shape != kv.k.shape or t.device != kv.k.device:
-            raise KernelError(f"{name} to read into are {tuple(t.shape)} on {t.device}, expected {tuple(kv.k.shape)} on {kv.k.device}")
-    call("gk_read8", kv._at, ptr(kv_len), ptr(slots), n, int(max_kv_len), int(last), ptr(out.k), ptr(out.v), stream_ptr())
+        if t.dtype is not _BFLOAT16 or t.shape != kv._sizes or t.get_device() != kv._index or not t.is_contiguous():
+            raise KernelError(f"{name} to read into must be contiguous bfloat16 {kv._sizes} on {kv.k.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    call("gk_read8", kv._at, kv_len.data_ptr(), slots.data_ptr(), n, int(max_kv_len), int(last), out.k.data_ptr(), out.v.data_ptr(), stream_ptr())
     return out
 
 
@@ -2574,7 +2590,8 @@ def _check_queries8(q: torch.Tensor, kv: PagedKV8, out: torch.Tensor | None) -> 
     if q.dim() != 3 or not q.is_cuda or not q.is_contiguous():
         raise KernelError(f"q must be a contiguous CUDA tensor [tokens, heads, head size], got {tuple(q.shape)} on {q.device}")
     _, n_kv, _, d = kv._sizes
-    if q.shape[2] != d or q.shape[1] % n_kv:
+    _, n_q, width = q.shape
+    if width != d or n_q % n_kv:
         raise KernelError(f"queries {tuple(q.shape)} do not fit pages of {n_kv} kv heads of {d}")
     if out is None:
         return torch.empty_like(q)
@@ -2644,8 +2661,8 @@ def _rows8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor | None, kv_len: tor
     n_seqs, n_q = kv_len.shape[0], q.shape[1]
     hint = min(kv_len_hint, window + max_q_len) if window else kv_len_hint
     rows, splits, pieces, scratch = _cut8(kv, max_q_len * (n_q // kv._sizes[1]), n_seqs, hint, cut)
-    call("gk_rows8", kv._at, ptr(q), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), n_seqs, n_q, max_q_len, rows, splits, pieces, ptr(scratch),
-         float(scale), int(window), int(sink), stream_ptr())
+    call("gk_rows8", kv._at, q.data_ptr(), out.data_ptr(), ptr(cu_q), kv_len.data_ptr(), slots.data_ptr(), n_seqs, n_q, max_q_len, rows, splits, pieces,
+         ptr(scratch), float(scale), int(window), bool(sink), stream_ptr())
     return out
 
 
@@ -2664,7 +2681,8 @@ def attention_decode8_fused(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: in
     rounded to bfloat16 on the way.  Returns ``[n_seqs, n_q, head_dim]``."""
     _check(qkv, "qkv", torch.bfloat16, 2)
     n = qkv.shape[0]
-    _check8(kv, qkv, ("kv_len", kv_len, n), ("slots", slots, n))
+    if not _fine8(kv, qkv, kv_len, slots, (n,)):
+        _check8(kv, qkv, ("kv_len", kv_len, n), ("slots", slots, n))
     if qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
         raise KernelError(f"qkv rows are {qkv.shape[1]} wide, expected {(n_q + 2 * n_kv) * head_dim}")
     if kv._sizes[1] != n_kv or kv._sizes[3] != head_dim or n_q % n_kv:
@@ -2688,7 +2706,8 @@ def attention_decode8(q: torch.Tensor, kv: PagedKV8, kv_len: torch.Tensor, slots
     here).  A sequence without tokens gets zeros."""
     out = _check_queries8(q, kv, out)
     n, n_q, d = q.shape
-    _check8(kv, q, ("kv_len", kv_len, n), ("slots", slots, n))
+    if not _fine8(kv, q, kv_len, slots, (n,)):
+        _check8(kv, q, ("kv_len", kv_len, n), ("slots", slots, n))
     _, n_kv, page, _ = kv._sizes
     if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and n_q // n_kv <= ROWS8_MAX_GROUP:
         return _rows8(q, kv, None, kv_len, slots, 1, max_kv_len, scale, window, sink, cut, out)
@@ -2741,7 +2760,8 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were; a token that sees no key gets zeros."""
     out = _check_queries8(q, kv, out)
     n_seqs = kv_len.shape[0]
-    _check8(kv, q, ("cu_q", cu_q, n_seqs + 1), ("kv_len", kv_len, n_seqs), ("slots", slots, n_seqs))
+    if not (_fine8(kv, q, kv_len, slots, (n_seqs,)) and _fine8(kv, q, cu_q, cu_q, (n_seqs + 1,))):
+        _check8(kv, q, ("cu_q", cu_q, n_seqs + 1), ("kv_len", kv_len, n_seqs), ("slots", slots, n_seqs))
     n_tokens, n_q, d = q.shape
     _, n_kv, page, _ = kv._sizes
     group = n_q // n_kv
