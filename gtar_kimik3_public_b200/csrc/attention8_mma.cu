@@ -38,7 +38,7 @@ struct Rows8 {
     const __nv_bfloat16* q;
     __nv_bfloat16* out;
     const int *cu_q, *kv_len, *slots;  // cu_q null: one token a sequence
-    int n_q, group, tiles, n_units;    // tiles: row tiles a sequence at most; a unit is a row tile of a sequence
+    int n_tokens, max_q_len, n_q, group, tiles, n_units;  // tiles: row tiles a sequence at most; a unit is a row tile of a sequence
     float sl2;                         // scale * log2(e)
     int window, sink;
     int n_splits;  // blocks of a cluster that share a (unit, kv head); 0: pieces of one size, about `pieces` of them
@@ -57,16 +57,25 @@ struct Fused8 : Norm8 {
 // A unit: which rows, which tokens, and the keys that some or all of them see.
 struct Unit {
     int seq, row_first, n_rows, first_token, past, slot, pos_low, begin, end, all_begin, tile_0, n_tiles;
+    bool sound;  // the sequence's length is one that the pages can hold
 };
 __device__ __forceinline__ Unit unit_of(const GkPages8& p, const Rows8& a, int unit, int most_rows) {
     Unit u;
     u.seq = a.cu_q ? unit / a.tiles : unit;
     u.row_first = a.cu_q ? (unit - u.seq * a.tiles) * most_rows : 0;
     // lengths, slots and the table are inputs of the step: they may be read while the kernel in front still runs
-    const int len = length_of(p, a.kv_len[u.seq]);
+    const int given = a.kv_len[u.seq], len = length_of(p, given);
+    u.sound = given == len;
     u.slot = a.slots[u.seq];
     u.first_token = a.cu_q ? a.cu_q[u.seq] : u.seq;
-    const int q_len = a.cu_q ? a.cu_q[u.seq + 1] - u.first_token : 1;
+    int q_len = a.cu_q ? a.cu_q[u.seq + 1] - u.first_token : 1;
+    if (a.cu_q) {  // tokens that there are none of, or more than the launch was made for: left out and recorded
+        const int most = u.first_token < 0 ? 0 : min(a.n_tokens - u.first_token, a.max_q_len);
+        if (q_len < 0 || q_len > most) {
+            if (p.error) *p.error = ERR_PLACE;
+            q_len = max(0, min(q_len, most));
+        }
+    }
     u.n_rows = min(most_rows, q_len * a.group - u.row_first);
     u.past = len - q_len;
     u.pos_low = u.past + u.row_first / a.group;  // of the first row
@@ -314,7 +323,7 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
     constexpr int ROWS = 8 * NT, KS = D / 16, MT = D / 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n_rows = u.n_rows, row_first = u.row_first, first_token = u.first_token, past = u.past, begin = u.begin;
-    const bool writes = FUSED && f.write_kv;
+    const bool writes = FUSED && f.write_kv && u.sound;
     const int end = u.end - (writes ? 1 : 0);  // the new key's place is not read
 
     // the numbers of the pages of this warp's next 32 tiles, one a lane
@@ -795,7 +804,7 @@ GK_EXPORT int gk_rows8_places(int head_dim, int rows, int cluster) {
 // Rows taken together: 8 or 16.  `splits` 1 .. 8: so many blocks, a cluster, share a (row tile, kv head); 0: the step's keys are cut into pieces of one
 // size, about `pieces` of them, with (pieces + units * n_kv) * rows * (head_dim + 3) floats of scratch, units = sequences * row tiles a sequence.
 // `q`, `out` [n_tokens][n_q][head_dim] bfloat16.  `max_q_len`: no sequence brings more tokens.
-static int rows8_entry(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_seqs, int n_q,
+static int rows8_entry(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_tokens, int n_seqs, int n_q,
                        int max_q_len, int rows, int splits, int pieces, float* scratch, float scale, int window, int sink, const Fused8& f, void* stream) {
     const int status = cache8::check(pages, "rows8");
     if (status != GK_OK) return status;
@@ -810,9 +819,9 @@ static int rows8_entry(const GkPages8* pages, const void* q, void* out, const in
     GK_REQUIRE((q || f.qkv) && out && kv_len && slots, "rows8: an array is missing");
     GK_REQUIRE((((uintptr_t)q | (uintptr_t)f.qkv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "rows8: memory must begin on 16-byte boundaries");
     const long long group = n_q / p.n_kv, tiles = cu_q ? (max_q_len * group + rows - 1) / rows : 1, units = tiles * n_seqs;
-    GK_REQUIRE(cu_q || (max_q_len == 1 && group <= rows), "rows8: %lld heads a kv head do not fit %d rows", group, rows);
+    GK_REQUIRE(n_tokens >= 0 && (cu_q || (max_q_len == 1 && n_tokens == n_seqs && group <= rows)), "rows8: %lld heads a kv head do not fit %d rows", group, rows);
     GK_REQUIRE(units <= 65535 && p.n_kv <= 65535 && pieces + units * p.n_kv < 2147483647LL, "rows8: grid too large");
-    const Rows8 a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, cu_q, kv_len, slots, n_q, (int)group, (int)tiles, (int)units, scale * 1.4426950408889634f,
+    const Rows8 a = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, cu_q, kv_len, slots, n_tokens, max_q_len, n_q, (int)group, (int)tiles, (int)units, scale * 1.4426950408889634f,
                      window, sink, splits, pieces, scratch, scratch ? scratch + (size_t)(pieces + units * p.n_kv) * rows * p.head_dim : nullptr};
     cudaStream_t s = (cudaStream_t)stream;
     if (f.qkv) {
@@ -823,9 +832,9 @@ static int rows8_entry(const GkPages8* pages, const void* q, void* out, const in
     return rows == 8 ? launch_rows8<128, 1, false>(p, a, f, s) : launch_rows8<128, 2, false>(p, a, f, s);
 }
 
-GK_EXPORT int gk_rows8(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_seqs, int n_q,
+GK_EXPORT int gk_rows8(const GkPages8* pages, const void* q, void* out, const int* cu_q, const int* kv_len, const int* slots, int n_tokens, int n_seqs, int n_q,
                        int max_q_len, int rows, int splits, int pieces, float* scratch, float scale, int window, int sink, void* stream) {
-    return rows8_entry(pages, q, out, cu_q, kv_len, slots, n_seqs, n_q, max_q_len, rows, splits, pieces, scratch, scale, window, sink, Fused8{}, stream);
+    return rows8_entry(pages, q, out, cu_q, kv_len, slots, n_tokens, n_seqs, n_q, max_q_len, rows, splits, pieces, scratch, scale, window, sink, Fused8{}, stream);
 }
 
 // One token a sequence, from the packed projection `qkv` [n_seqs][(n_q + 2 n_kv) * head_dim] bfloat16: norm and rotation of queries and keys and the
@@ -841,5 +850,5 @@ GK_EXPORT int gk_rows8_fused(const GkPages8* pages, const void* qkv, const void*
                table_positions);
     GK_REQUIRE((((uintptr_t)wq | (uintptr_t)wk | (uintptr_t)cos_table | (uintptr_t)sin_table) & 15) == 0, "rows8_fused: weights and tables must begin on 16-byte boundaries");
     const Fused8 f = {{wq, wk, cos_table, sin_table, table_positions, use_norm, eps}, (const __nv_bfloat16*)qkv, weight_dtype == GK_BF16, write_kv};
-    return rows8_entry(pages, nullptr, out, nullptr, kv_len, slots, n_seqs, n_q, 1, rows, splits, pieces, scratch, scale, window, 0, f, stream);
+    return rows8_entry(pages, nullptr, out, nullptr, kv_len, slots, n_seqs, n_seqs, n_q, 1, rows, splits, pieces, scratch, scale, window, 0, f, stream);
 }

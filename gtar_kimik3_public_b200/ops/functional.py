@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .library import KernelError, call, current_device, dtype_code, library, ptr, require_device, stream_ptr
+from .library import KernelError, call, current_device, dtype_code, in_order, library, ptr, require_device, stream_ptr
 
 
 def _check(tensor: torch.Tensor, name: str, dtype=None, dims: int | None = None) -> None:
@@ -2661,7 +2661,7 @@ def _rows8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor | None, kv_len: tor
     n_seqs, n_q = kv_len.shape[0], q.shape[1]
     hint = min(kv_len_hint, window + max_q_len) if window else kv_len_hint
     rows, splits, pieces, scratch = _cut8(kv, max_q_len * (n_q // kv._sizes[1]), n_seqs, hint, cut)
-    call("gk_rows8", kv._at, q.data_ptr(), out.data_ptr(), ptr(cu_q), kv_len.data_ptr(), slots.data_ptr(), n_seqs, n_q, max_q_len, rows, splits, pieces,
+    call("gk_rows8", kv._at, q.data_ptr(), out.data_ptr(), ptr(cu_q), kv_len.data_ptr(), slots.data_ptr(), q.shape[0], n_seqs, n_q, max_q_len, rows, splits, pieces,
          ptr(scratch), float(scale), int(window), bool(sink), stream_ptr())
     return out
 
@@ -2738,6 +2738,10 @@ def rows8_wins(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, n_kv
     return rows < prefill
 
 
+# The prefill kernels read lengths and slots, inputs of a step elsewhere, before they wait for the kernel in front, which here is the one that writes them.
+_attention_prefill_in_order = in_order(attention_prefill)
+
+
 def _clean_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, last: int) -> tuple[PagedKV, torch.Tensor, torch.Tensor]:
     """The step's pages as bfloat16 with a table, lengths and slots of their own.  Where the sequences could have more pages than there are, pages keep
     their numbers."""
@@ -2757,7 +2761,7 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
                        scale: float, window: int = 0, sink: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the packed new tokens ``q [n_tokens, n_q, d]`` (bfloat16 or float32) over 8-bit pages.  Sequence ``i`` owns the tokens
     ``cu_q[i] .. cu_q[i+1]-1``, its last positions: ``kv_len[i]`` counts its cached tokens including them.  ``max_q_len`` and ``max_kv_len`` are the
-    largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were; a token that sees no key gets zeros."""
+    largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were."""
     out = _check_queries8(q, kv, out)
     n_seqs = kv_len.shape[0]
     if not (_fine8(kv, q, kv_len, slots, (n_seqs,)) and _fine8(kv, q, cu_q, cu_q, (n_seqs + 1,))):
@@ -2769,7 +2773,7 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
         if rows8_wins(n_tokens, n_seqs, max_q_len, min(max_kv_len, window + max_q_len) if window else max_kv_len, n_kv, group, d, _sm_count_of(kv._index)):
             return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
         pages, lens, own_slots = _clean_pages8(kv, kv_len, slots, max_kv_len, window + max_q_len if window else 0)
-        return attention_prefill(q, pages, cu_q, lens, own_slots, max_q_len, scale, window, out, sink=sink)
+        return _attention_prefill_in_order(q, pages, cu_q, lens, own_slots, max_q_len, scale, window, out, sink=sink)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
          int(window), int(sink), stream_ptr())
     return out

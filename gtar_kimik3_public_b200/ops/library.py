@@ -114,7 +114,7 @@ _SIGNATURES: dict[str, list] = {
     "gk_memory_scan": [P, I, L, I, I, I, I, I, P, F, P, P, P, P, P, P, P, I, I, I, I, P],
     "gk_write8": [P, P, I, P, P, I, I, F, P, P, I, I, P, P, P, I, P, I, I, I, P],
     "gk_read8": [P, P, P, I, I, I, P, P, P],
-    "gk_rows8": [P, P, P, P, P, P, I, I, I, I, I, I, P, F, I, I, P],
+    "gk_rows8": [P, P, P, P, P, P, I, I, I, I, I, I, I, P, F, I, I, P],
     "gk_rows8_fused": [P, P, P, P, I, I, F, P, P, I, I, I, P, P, P, I, I, I, I, I, P, F, I, P],
     "gk_rows8_places": [I, I, I],
     "gk_clean8": [P, P, P, I, I, I, I, P, P, P, P, P, P],

@@ -447,6 +447,55 @@ def test_page_numbers_slots_and_lengths_that_cannot_be(few, monkeypatch):
         assert torch.equal(kv.k.view(torch.uint8), before)
 
 
+def test_tokens_that_there_are_none_of(monkeypatch):
+    """Starts beyond the queries, starts that fall, and more tokens than ``max_q_len``: left out and reported by the kernel for few rows."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: True)
+    kv, slots, table = sequences([100, 90], 2, 128)
+    q = rand(8, 4, 128, seed=5).to(torch.bfloat16).to(DEV)
+    good = F().attention_prefill8(q, kv, ints(0, 4, 8), ints(100, 90), slots, 4, 100, 0.1)
+    F().check_kernel_errors(DEV)
+    for cu, most, kept in (([0, 4, 900], 4, 8), ([0, 4, 2], 4, 4), ([-3, 4, 8], 4, None), ([0, 4, 8], 2, None)):
+        out = torch.full(q.shape, 5.0, dtype=q.dtype, device=DEV)
+        F().attention_prefill8(q, kv, ints(*cu), ints(100, 90), slots, most, 100, 0.1, out=out)
+        with pytest.raises(Exception, match="page number"):
+            F().check_kernel_errors(DEV)
+        if kept is not None:
+            assert torch.equal(out[:4], good[:4]) and (kept == 8 or (out[4:] == 5.0).all())
+
+
+def test_a_length_that_cannot_be_writes_nothing():
+    kv, slots, table = sequences([100, 90], 2, 128)
+    before = [t.view(torch.uint8).clone() for t in (kv.k, kv.v, kv.k_exp, kv.v_exp)]
+    qkv = rand(2, 8 * 128).to(torch.bfloat16).to(DEV)
+    for wrong in (10**6, 0, -4):
+        F().attention_decode8_fused(qkv, 4, 2, 128, None, None, 1.0, None, None, kv, ints(wrong, wrong), slots, 99, 100, 0.1)
+        if wrong:
+            with pytest.raises(Exception, match="page number"):
+                F().check_kernel_errors(DEV)
+        assert all(torch.equal(a, t.view(torch.uint8)) for a, t in zip(before, (kv.k, kv.v, kv.k_exp, kv.v_exp)))
+
+
+def test_which_kernels_start_early(monkeypatch):
+    """Prefill attention over pages made clean reads what the kernel in front writes, before it waits: it never starts early.  The kernel that joins
+    pieces touches nothing before it waits."""
+    from tests.test_early_launches import _early_edges
+
+    kv, slots, table = sequences([300, 200], 2, 128)
+    q = rand(120, 4, 128, seed=5).to(torch.bfloat16).to(DEV)
+    lens, cu = ints(300, 200), ints(0, 60, 120)
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: False)
+    prompts = lambda: F().attention_prefill8(q, kv, cu, lens, slots, 60, 300, 0.1)  # noqa: E731
+    pieces = lambda: F().attention_decode8(q[:2], kv, lens, slots, 300, 0.1, cut=(0, 40))  # noqa: E731
+    want = prompts().clone(), pieces().clone()
+    before = F().set_pdl(True)
+    try:
+        edges = [_early_edges(run) for run in (prompts, pieces)]
+    finally:
+        F().set_pdl(before)
+    assert edges == [(1, 0), (1, 1)]
+    assert torch.equal(prompts(), want[0]) and torch.equal(pieces(), want[1])
+
+
 def test_refusals():
     f = F()
     kv, slots, _ = empty_pages(2, 100, 2, 64)
