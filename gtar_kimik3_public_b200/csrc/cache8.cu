@@ -319,11 +319,12 @@ int launch_write8(const GkPages8& p, const Write8& a, cudaStream_t stream) {
 }
 
 // ------------------------------------------------------------------ read back
-// For attention over what was read: pages renumbered under a table, lengths and slots of their own, so that no number that cannot be reaches it; and
+// For attention over what was read: pages renumbered under a table, lengths, slots and starts of their own, so that no number that cannot be reaches it; and
 // a row of values that holds a NaN becomes zeros with a NaN key, which a token that does not see it cannot meet (0 * NaN).
 struct Clean8 {
-    int *table, *kv_len, *slots;  // [n_seqs][per], [n_seqs], [n_seqs]; null: read back under the pages' own numbers
-    int per, own_numbers;         // pages a sequence; whether a page keeps its number or is seq * per + index
+    int *table, *kv_len, *slots, *cu_q;  // [n_seqs][per], [n_seqs], [n_seqs], [n_seqs + 1]
+    const int* cu_q_in;
+    int n_tokens, per, own_numbers;  // pages a sequence; whether a page keeps its number or is seq * per + index
 };
 
 // N numbers of a row as bfloat16: e4m3 times a power of two, exact.
@@ -347,6 +348,23 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
     pdl_wait();
     const int seq = blockIdx.y, index = blockIdx.x, hk = blockIdx.z, d = HD ? HD : p.head_dim;
     int len = length_of(p, kv_len[seq]);
+    if (CLEAN && seq == 0 && index == 0 && hk == 0 && threadIdx.x < 32) {  // starts within the queries, none before the one in front
+        int before = 0;
+        for (int base = 0; base <= (int)gridDim.y; base += 32) {
+            const int i = base + threadIdx.x, given = i <= (int)gridDim.y ? clean.cu_q_in[i] : 0;
+            int at = max(before, min(max(given, 0), clean.n_tokens));
+#pragma unroll
+            for (int w = 1; w < 32; w <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, at, w);
+                if ((int)threadIdx.x >= w) at = max(at, other);
+            }
+            if (i <= (int)gridDim.y) {
+                clean.cu_q[i] = at;
+                if (at != given && p.error) *p.error = ERR_PLACE;
+            }
+            before = __shfl_sync(0xffffffffu, at, 31);
+        }
+    }
     if (CLEAN && len > (long long)clean.per * p.page_size) {
         if (p.error) *p.error = ERR_PLACE;
         len = clean.per * p.page_size;
@@ -474,14 +492,15 @@ GK_EXPORT int gk_read8(const GkPages8* pages, const int* kv_len, const int* slot
 }
 
 // The same for attention over what is read: `per` pages a sequence under numbers seq * per + index (`own_numbers`: their own), and `table`
-// [n_seqs][per], `len_out` and `slots_out` [n_seqs] to go with them.  Heads of 64 or 128.
-GK_EXPORT int gk_clean8(const GkPages8* pages, const int* kv_len, const int* slots, int n_seqs, int per, int own_numbers, int last, void* k_out, void* v_out,
-                        int* table, int* len_out, int* slots_out, void* stream) {
+// [n_seqs][per], `len_out` and `slots_out` [n_seqs] and `cu_out` [n_seqs + 1] to go with them.  Heads of 64 or 128.
+GK_EXPORT int gk_clean8(const GkPages8* pages, const int* cu_q, const int* kv_len, const int* slots, int n_tokens, int n_seqs, int per, int own_numbers,
+                        int last, void* k_out, void* v_out, int* table, int* len_out, int* slots_out, int* cu_out, void* stream) {
     const int status = cache8::check(pages, "clean8");
     if (status != GK_OK) return status;
     GK_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && per > 0 && last >= 0 && (long long)n_seqs * per < 2147483647LL, "clean8: bad sizes n_seqs=%d per=%d last=%d",
                n_seqs, per, last);
     if (n_seqs == 0) return GK_OK;
-    GK_REQUIRE(kv_len && slots && k_out && v_out && table && len_out && slots_out, "clean8: an array is missing");
-    return launch_read8<true>(*pages, kv_len, slots, n_seqs, per, last, k_out, v_out, Clean8{table, len_out, slots_out, per, own_numbers}, (cudaStream_t)stream);
+    GK_REQUIRE(cu_q && kv_len && slots && k_out && v_out && table && len_out && slots_out && cu_out, "clean8: an array is missing");
+    return launch_read8<true>(*pages, kv_len, slots, n_seqs, per, last, k_out, v_out,
+                              Clean8{table, len_out, slots_out, cu_out, cu_q, n_tokens, per, own_numbers}, (cudaStream_t)stream);
 }

@@ -2742,19 +2742,20 @@ def rows8_wins(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, n_kv
 _attention_prefill_in_order = in_order(attention_prefill)
 
 
-def _clean_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, last: int) -> tuple[PagedKV, torch.Tensor, torch.Tensor]:
-    """The step's pages as bfloat16 with a table, lengths and slots of their own.  Where the sequences could have more pages than there are, pages keep
-    their numbers."""
+def _clean_pages8(kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, n_tokens: int, max_kv_len: int,
+                  last: int) -> tuple[PagedKV, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The step's pages as bfloat16 with a table, starts, lengths and slots of their own.  Where the sequences could have more pages than there
+    are, pages keep their numbers."""
     n, device = kv_len.shape[0], kv.k.device
     per = min(max(1, -(-int(max_kv_len) // kv.page_size)), kv.max_pages)
     own_numbers = n * per > kv.k.shape[0]
     shape = (kv.k.shape[0] if own_numbers else n * per, *kv.k.shape[1:])
     k, v = (torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(2))
-    ints = torch.empty((n * per + 2 * n,), dtype=torch.int32, device=device)
-    table, lens, own_slots = ints[: n * per].view(n, per), ints[n * per: n * per + n], ints[n * per + n:]
-    call("gk_clean8", kv._at, ptr(kv_len), ptr(slots), n, per, int(own_numbers), int(last), ptr(k), ptr(v), ptr(table), ptr(lens), ptr(own_slots),
-         stream_ptr())
-    return PagedKV(k, v, table), lens, own_slots
+    table, lens, own_slots, starts = torch.empty((n * per + 3 * n + 1,), dtype=torch.int32, device=device).split([n * per, n, n, n + 1])
+    table = table.view(n, per)
+    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), n_tokens, n, per, int(own_numbers), int(last), ptr(k), ptr(v), ptr(table), ptr(lens),
+         ptr(own_slots), ptr(starts), stream_ptr())
+    return PagedKV(k, v, table), starts, lens, own_slots
 
 
 def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, max_kv_len: int,
@@ -2772,8 +2773,8 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and group <= ROWS8_MAX_GROUP and n_seqs and n_tokens:
         if rows8_wins(n_tokens, n_seqs, max_q_len, min(max_kv_len, window + max_q_len) if window else max_kv_len, n_kv, group, d, _sm_count_of(kv._index)):
             return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
-        pages, lens, own_slots = _clean_pages8(kv, kv_len, slots, max_kv_len, window + max_q_len if window else 0)
-        return _attention_prefill_in_order(q, pages, cu_q, lens, own_slots, max_q_len, scale, window, out, sink=sink)
+        pages, starts, lens, own_slots = _clean_pages8(kv, cu_q, kv_len, slots, n_tokens, max_kv_len, window + max_q_len if window else 0)
+        return _attention_prefill_in_order(q, pages, starts, lens, own_slots, max_q_len, scale, window, out, sink=sink)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
          int(window), int(sink), stream_ptr())
     return out

@@ -447,6 +447,21 @@ def test_page_numbers_slots_and_lengths_that_cannot_be(few, monkeypatch):
         assert torch.equal(kv.k.view(torch.uint8), before)
 
 
+def test_starts_that_cannot_be_behind_clean_pages(monkeypatch):
+    """Starts beyond the queries and starts that fall: put within the queries and in order, and reported."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: False)
+    kv, slots, table = sequences([100, 90], 2, 128)
+    q = rand(80, 4, 128, seed=5).to(torch.bfloat16).to(DEV)
+    good = F().attention_prefill8(q, kv, ints(0, 40, 80), ints(100, 90), slots, 40, 100, 0.1)
+    F().check_kernel_errors(DEV)
+    for cu in ([0, 40, 9000], [0, 40, 20]):
+        out = torch.full(q.shape, 5.0, dtype=q.dtype, device=DEV)
+        F().attention_prefill8(q, kv, ints(*cu), ints(100, 90), slots, 40, 100, 0.1, out=out)
+        with pytest.raises(Exception, match="page number"):
+            F().check_kernel_errors(DEV)
+        assert torch.equal(out[:40], good[:40]) and (torch.equal(out[40:], good[40:]) if cu[2] > 80 else (out[40:] == 5.0).all())
+
+
 def test_tokens_that_there_are_none_of(monkeypatch):
     """Starts beyond the queries, starts that fall, and more tokens than ``max_q_len``: left out and reported by the kernel for few rows."""
     monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: True)
