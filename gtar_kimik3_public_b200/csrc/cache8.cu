@@ -300,8 +300,9 @@ __global__ void __launch_bounds__(128, 4) write8_stream_kernel(const GkPages8 p,
 
 template <int HD, typename TW>
 int launch_write8(const GkPages8& p, const Write8& a, cudaStream_t stream) {
-    // Sixteen rows a task would leave the device idle where rows are few: four below eight warps' worth of sixteen an SM.
-    const bool many = (long long)a.n_tokens * (a.n_q + 2 * p.n_kv) >= 148 * 8 * 16;
+    // Warps that stay have a ring to fill first.  us, four rows a warp / warps that stay: 16,384 rows of 128 7.4 / 9.7, 49,152 11.7 / 13.3, 65,536 15.6 / 14.8,
+    // 196,608 40 / 31; 40,960 rows of 64 8.5 / 9.0, 81,920 13.1 / 14.4.
+    const bool many = (long long)a.n_tokens * (a.n_q + 2 * p.n_kv) * HD >= 7 << 20;
     const int per = many ? 4 * STREAM_R : 4, q_tasks = (a.n_q + per - 1) / per, tasks = q_tasks + (a.write_kv ? (2 * p.n_kv + per - 1) / per : 0);
     const long long n_tasks = (long long)a.n_tokens * tasks, blocks = (n_tasks + 3) / 4;
     GK_REQUIRE(n_tasks + 148 * 4 * 4 * 3 < 4294967295LL, "write8: too many tokens");

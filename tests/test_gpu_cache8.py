@@ -114,17 +114,18 @@ def test_write(dtype, n_q, n_kv, d, norm, rope):
         assert (getattr(kv, name + "_exp").cpu()[untouched] == 255).all()
 
 
-@pytest.mark.parametrize("n_q,n_kv,d,lens", [(16, 8, 128, [700, 1, 65]), (6, 2, 64, [1500, 800]), (3, 3, 128, [2300])])
+@pytest.mark.parametrize("n_q,n_kv,d,lens", [(16, 8, 128, [700, 1, 65]), (6, 2, 64, [1500, 800]), (3, 3, 128, [2300]),
+                                             (16, 8, 128, [1500, 1, 400]), (6, 2, 64, [8000, 3500]), (3, 3, 128, [6400])])
 @pytest.mark.parametrize("norm", [True, False])
 def test_write_of_many_tokens(n_q, n_kv, d, lens, norm):
-    """Enough rows for the warps that stay.  Keys are the formula in 64 bits rounded once, all of them; a place outside the pages is left out and
+    """Too few rows for the warps that stay, and enough.  Keys are the formula in 64 bits rounded once, all of them; a place outside the pages is left out and
     reported, the others are what they are."""
     past, eps = [5 * i for i in range(len(lens))], 1e-6
     kv, slots, table = empty_pages(len(lens), max(lens) + 20, n_kv, d)
     pos = [p + i for n, p in zip(lens, past) for i in range(n)]
     seq = [i for i, n in enumerate(lens) for _ in range(n)]
     qkv = rand(len(pos), (n_q + 2 * n_kv) * d, seed=2).to(torch.bfloat16)
-    assert len(pos) * (n_q + 2 * n_kv) >= 148 * 8 * 16
+    assert (len(pos) * (n_q + 2 * n_kv) * d >= 7 << 20) == (sum(lens) > (1900 if n_kv == 8 else 2300))
     wq, wk = (1 + 0.1 * rand(d, seed=20)).to(torch.bfloat16), (1 + 0.1 * rand(d, seed=21)).to(torch.bfloat16)
     cos, sin = plain.rotary_tables(torch.arange(max(pos) + 1), d, 1e4)
     cos, sin = cos[:, : d // 2].float().contiguous(), sin[:, : d // 2].float().contiguous()
@@ -265,6 +266,20 @@ def test_decode(dtype, cut, n_q, n_kv, d, window, sink):
             k, v = held(kv, table, int(slots[i]), n)
             check_attention(got[i:i + 1], q[i:i + 1], k, v, n - 1, window, sink, SINGLE[dtype], f"sequence of {n}")
     F().check_kernel_errors(DEV)
+
+
+@pytest.mark.parametrize("page", [32, 96])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_other_pages(page, dtype):
+    n_q, n_kv, d, lens = 4, 2, 128, [100, 32, 97]
+    kv, slots, table = sequences(lens, n_kv, d, page)
+    q = rand(9, n_q, d, seed=5).to(dtype)
+    one = F().attention_decode8(q[:3].contiguous().to(DEV), kv, ints(*lens), slots, 100, d**-0.5)
+    several = F().attention_prefill8(q.to(DEV), kv, ints(0, 3, 6, 9), ints(*lens), slots, 3, 100, d**-0.5)
+    for i, m in enumerate(lens):
+        k, v = held(kv, table, int(slots[i]), m)
+        check_attention(one[i:i + 1], q[i:i + 1], k, v, m - 1, 0, False, SINGLE[dtype], f"sequence of {m}")
+        check_attention(several[3 * i:3 * i + 3], q[3 * i:3 * i + 3], k, v, m - 3, 0, False, SEVERAL[dtype], f"sequence of {m}")
 
 
 @pytest.mark.parametrize("n_q,n_kv,d", [(16, 8, 128), (8, 1, 128), (12, 1, 128), (16, 1, 64), (6, 2, 64), (1, 1, 64)])

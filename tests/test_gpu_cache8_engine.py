@@ -124,3 +124,72 @@ def test_trace_run(tmp_path, monkeypatch):
     standard = (plain_logits8(tag, tokens, "lowp", monkeypatch)[69:] - oracle).abs().max().item()
     got = torch.stack([torch.from_numpy(np.fromfile(tmp_path / f"{i}.f32", dtype="<f4")) for i in range(11)])
     assert (got.double() - oracle).abs().max().item() <= 2 * standard + 1e-4
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_an_attention_layer_with_a_window(dtype, d, monkeypatch):
+    """Pages go back to the pool as the window leaves them and are used again by another sequence; prompts, pieces and single tokens."""
+    from dataclasses import replace
+
+    from gtar_kimik3_public_b200.cache import Cache, CacheLayout
+    from gtar_kimik3_public_b200.engine.step import SequenceStep, plan_step
+    from gtar_kimik3_public_b200.parts import build_part
+    from tests.test_gpu_kernels import DEV, rand
+    from tests.test_gpu_parts import load_part
+
+    hidden, n_q, n_kv, window, eps, theta, n = 96, 4, 2, 70, 1e-5, 1e4, 260
+    rope = build_part("position", "rope", dim=d, base=theta)
+    mixer = build_part("mixer", "gqa_attention", hidden_size=hidden, n_q_heads=n_q, n_kv_heads=n_kv, head_dim=d, qk_norm_eps=eps, position=rope, window=window)
+    w = {"q_proj.weight": rand(n_q * d, hidden, seed=1, scale=0.1), "k_proj.weight": rand(n_kv * d, hidden, seed=2, scale=0.1),
+         "v_proj.weight": rand(n_kv * d, hidden, seed=3, scale=0.1), "o_proj.weight": rand(hidden, n_q * d, seed=4, scale=0.1),
+         "q_norm.weight": 1 + 0.1 * rand(d, seed=5), "k_norm.weight": 1 + 0.1 * rand(d, seed=6)}
+    w = {k: v.to(torch.bfloat16).double() if "proj" in k else v.float().double() for k, v in w.items()}
+    load_part(mixer, w, dtype)
+    rope.prepare(n, torch.device(DEV))
+    request = replace(mixer.cache_request(), dtype=torch.float8_e4m3fn)
+    cache = Cache(CacheLayout([request]), 64 * 9, dtype, DEV, max_seqs=2)
+    group, = cache.kv_groups
+    for t in (group.k, group.v):
+        t.view(torch.uint8).fill_(0x7F)
+    group.k_exp.fill_(255)
+    group.v_exp.fill_(255)
+    xs = [rand(n, hidden, seed=7 + i).to(dtype) for i in range(2)]
+    slots, at, rows = [cache.open(), cache.open()], [0, 0], [[], []]
+    pieces = [[100, 3, 64] + [1] * 93, [1] * 90 + [33, 70] + [1] * 67]
+    for step in range(max(map(len, pieces))):
+        live = [i for i in range(2) if step < len(pieces[i])]
+        sequences = [SequenceStep(slots[i], cache.grow(slots[i], pieces[i][step]), [0] * pieces[i][step], []) for i in live]
+        cache.sync()
+        ctx = plan_step(sequences, dtype, torch.device(DEV), 1)
+        x = torch.cat([xs[i][at[i]:at[i] + pieces[i][step]] for i in live]).to(DEV)
+        out, row = mixer.forward(x, ctx, cache.view(0)).double().cpu(), 0
+        for i in live:
+            m = pieces[i][step]
+            rows[i].append(out[row:row + m])
+            at[i], row = at[i] + m, row + m
+    cache.check_invariants()
+    assert len(group.owned[slots[0]]) <= 3  # what the window has left went back
+    cfg = {"num_attention_heads": n_q, "num_key_value_heads": n_kv, "head_dim": d, "rms_norm_eps": eps, "rope_theta": theta}
+    attend = plain.causal_gqa_attention
+
+    def wanted(x, keep8, lowp):
+        with monkeypatch.context() as patch:
+            as_kept = plain8.quantised if keep8 else (lambda t: t)
+            patch.setattr(plain, "causal_gqa_attention", lambda q, k, v: attend(q, as_kept(k), as_kept(v), window))
+            if lowp:
+                patch.setattr(plain, "LOWP", torch.bfloat16)
+                return plain.attention_mixer(x.float(), {k: v.float() for k, v in w.items()}, "", cfg).double()
+            return plain.attention_mixer(x.double(), w, "", cfg)
+
+    for i in range(2):
+        got, oracle = torch.cat(rows[i]), wanted(xs[i], True, False)
+        assert got.shape[0] == sum(pieces[i]) and torch.isfinite(got).all()
+        oracle = oracle[: got.shape[0]]
+        err = (got - oracle).abs().max().item()
+        if dtype == torch.float32:  # as for whole models: a few roundings that lie between two numbers
+            moved = (oracle - wanted(xs[i], False, False)[: got.shape[0]]).abs().max().item()
+            assert err < 1e-4 + 0.1 * moved
+        else:
+            standard = (wanted(xs[i], True, True)[: got.shape[0]] - oracle).abs().max().item()
+            assert err <= 2 * standard + 1e-4
