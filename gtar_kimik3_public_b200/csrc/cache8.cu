@@ -387,13 +387,17 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
         return;
     }
     const int rows = page < 0 ? 0 : min(p.page_size, len - index * p.page_size);
+    // Under its own number a page may be another, longer sequence's too: what lies behind this one's end is made as that one makes it, where there is
+    // a power that the write makes.  (The prefill kernels set hidden keys' scores aside, and hidden values are finite.)
+    const bool all = CLEAN && clean.own_numbers;
+    const auto kept = [](int b) { return (unsigned)(b - 127 - LOW) <= (unsigned)(HIGH - LOW); };
     const size_t from = ((size_t)max(page, 0) * p.n_kv + hk) * p.page_size, to = ((size_t)to_page * p.n_kv + hk) * p.page_size;
     if constexpr (HD > 0) {
         constexpr int LANES = HD / 16;
         const int c = threadIdx.x % LANES * 16;
         for (int row = threadIdx.x / LANES; row < p.page_size; row += 256 / LANES) {
             uint32_t k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (row < rows) {
+            if (row < rows || (all && kept(p.k_exp[from + row]) && kept(p.v_exp[from + row]))) {
                 const uint4 x = *reinterpret_cast<const uint4*>(p.k + (from + row) * HD + c), y = *reinterpret_cast<const uint4*>(p.v + (from + row) * HD + c);
                 const uint32_t ks[4] = {x.x, x.y, x.z, x.w}, vs[4] = {y.x, y.y, y.z, y.w};
                 widen<16>(ks, power_of(p.k_exp[from + row]), k);

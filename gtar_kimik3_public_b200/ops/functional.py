@@ -2561,8 +2561,8 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
         q_out = torch.empty((n, n_q, head_dim), dtype=qkv.dtype, device=qkv.device)
     else:
         _check(q_out, "q_out", qkv.dtype, 3)
-        if q_out.shape != (n, n_q, head_dim):
-            raise KernelError(f"q_out is {tuple(q_out.shape)}, expected {(n, n_q, head_dim)}")
+        if q_out.shape != (n, n_q, head_dim) or q_out.get_device() != kv._index:
+            raise KernelError(f"q_out is {tuple(q_out.shape)} on {q_out.device}, expected {(n, n_q, head_dim)} on {kv.k.device}")
     call("gk_write8", kv._at, qkv.data_ptr(), code, ptr(q_weight), ptr(k_weight), weight_code, q_weight is not None, float(eps), ptr(cos), ptr(sin),
          table_positions, int(max_position), tok_pos.data_ptr(), tok_seq.data_ptr(), slots.data_ptr(), slots.shape[0], q_out.data_ptr(), n, n_q, bool(write_kv),
          stream_ptr())
@@ -2572,7 +2572,8 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
 def read_pages8(kv: PagedKV8, kv_len: torch.Tensor, slots: torch.Tensor, max_kv_len: int, out: PagedKV | None = None, last: int = 0) -> PagedKV:
     """The 8-bit pages of the listed sequences read back, exactly, as bfloat16 pages of the same numbers: those that hold each sequence's last
     ``last`` positions (0: all).  Places behind a sequence's end in its last page become zero; pages that the step does not name are left as they
-    were (in pages made here, ``out`` None: undefined).  ``out``: pages of the same shape; ``max_kv_len``: the longest of ``kv_len``, known on the host."""
+    were (in pages made here, ``out`` None: undefined).  ``out``: pages of the same shape; ``max_kv_len``: the longest of ``kv_len``, known on the host.  A page that
+    two of the sequences share has to be full in both."""
     n = kv_len.shape[0]
     if not _fine8(kv, kv_len, kv_len, slots, (n,)):
         _check8(kv, kv_len, ("kv_len", kv_len, n), ("slots", slots, n))
@@ -2678,7 +2679,7 @@ def attention_decode8_fused(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: in
                             cut: tuple[int, int] | None = None) -> torch.Tensor:
     """``qk_norm_rope_write8`` and ``attention_decode8`` of one new token per sequence in one kernel, from the packed projection
     ``qkv [n_seqs, (n_q + 2 n_kv) * head_dim]`` (bfloat16, heads of 64 or 128, pages of 64).  The cache gets the same bytes; the queries are not
-    rounded to bfloat16 on the way.  Returns ``[n_seqs, n_q, head_dim]``."""
+    rounded to bfloat16 on the way.  No two sequences of the call may write into one page (with ``write_kv``, a slot stands in it once).  Returns ``[n_seqs, n_q, head_dim]``."""
     _check(qkv, "qkv", torch.bfloat16, 2)
     n = qkv.shape[0]
     if not _fine8(kv, qkv, kv_len, slots, (n,)):
@@ -2773,7 +2774,7 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and group <= ROWS8_MAX_GROUP and n_seqs and n_tokens:
         if rows8_wins(n_tokens, n_seqs, max_q_len, min(max_kv_len, window + max_q_len) if window else max_kv_len, n_kv, group, d, _sm_count_of(kv._index)):
             return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
-        pages, starts, lens, own_slots = _clean_pages8(kv, cu_q, kv_len, slots, n_tokens, max_kv_len, window + max_q_len if window else 0)
+        pages, starts, lens, own_slots = _clean_pages8(kv, cu_q, kv_len, slots, n_tokens, max_kv_len, window + max_q_len if 0 < window < max_kv_len else 0)
         return _attention_prefill_in_order(q, pages, starts, lens, own_slots, max_q_len, scale, window, out, sink=sink)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
          int(window), int(sink), stream_ptr())

@@ -418,6 +418,37 @@ def test_prefill_where_pages_keep_their_numbers(monkeypatch):
     F().check_kernel_errors(DEV)
 
 
+@pytest.mark.parametrize("n_q,n_kv,d", [(4, 2, 128), (6, 2, 64)])
+def test_prefill_where_sequences_share_pages(n_q, n_kv, d, monkeypatch):
+    """The same slot at two lengths that end inside one page, and another sequence that begins with its first page: under their own numbers the pages serve
+    all of them."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: False)
+    new, lens = [70, 1, 40, 5], [200, 180, 130, 170]
+    kv, slots, table = sequences([200, 200, 200, 200], n_kv, d)
+    whole = kv.block_table.clone()
+    whole[slots[2], 0] = whole[slots[0], 0]
+    slots = torch.stack([slots[0], slots[0], slots[2], slots[0]])
+    narrow = F().PagedKV8(kv.k, kv.v, kv.k_exp, kv.v_exp, whole)
+    wide = F().PagedKV8(kv.k, kv.v, kv.k_exp, kv.v_exp, torch.cat([whole, torch.zeros((whole.shape[0], 60), dtype=torch.int32, device=DEV)], 1).contiguous())
+    q = rand(116, n_q, d, seed=5).to(torch.bfloat16).to(DEV)
+    args = (ints(0, 70, 71, 111, 116), ints(*lens), slots, 70)
+    want = F().attention_prefill8(q, narrow, *args, 200, d**-0.5)
+    for _ in range(5):
+        assert torch.equal(F().attention_prefill8(q, wide, *args, 64 * 60, d**-0.5), want)
+    F().check_kernel_errors(DEV)
+
+
+def test_a_window_longer_than_any_sequence(monkeypatch):
+    """As if there were none, up to the largest number that a window can be."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: False)
+    kv, slots, _ = sequences([200, 64], 2, 128)
+    q = rand(71, 4, 128, seed=5).to(torch.bfloat16).to(DEV)
+    args = (ints(0, 70, 71), ints(200, 64), slots, 70, 200, 0.1)
+    want = F().attention_prefill8(q, kv, *args)
+    for window in (200, 2**31 - 71, 2**31 - 1):
+        assert torch.equal(F().attention_prefill8(q, kv, *args, window), want)
+
+
 @pytest.mark.parametrize("few", [True, False])
 def test_page_numbers_slots_and_lengths_that_cannot_be(few, monkeypatch):
     """They are skipped and reported; the step's other sequences are what they are."""
@@ -543,6 +574,7 @@ def test_refusals():
     refused("entries", lambda: f.attention_decode8(q, kv, lens[:1], slots, 100, 0.1))
     refused("int32", lambda: f.attention_decode8(q, kv, lens.long(), slots, 100, 0.1))
     refused("window", lambda: f.attention_decode8(q, kv, lens, slots, 100, 0.1, -1))
+    refused("window", lambda: f.attention_prefill8(q, kv, ints(0, 1, 2), lens, slots, 1, 100, 0.1, -1))
     refused("on cpu", lambda: f.attention_decode8(q, kv, lens.cpu(), slots, 100, 0.1))
     refused("like q", lambda: f.attention_decode8(q, kv, lens, slots, 100, 0.1, out=q.float()))
     refused("entries", lambda: f.attention_prefill8(q, kv, ints(0, 2), lens, slots, 1, 100, 0.1))
