@@ -924,19 +924,22 @@ def attention_prefill(
         raise KernelError(f"tensor_cores must be auto, tcgen05 or mma, got {tensor_cores!r}")
     if tensor_cores == "tcgen05" and d != 128:
         raise KernelError("the tcgen05 prefill attention takes head size 128 only")
-    if tensor_cores == "tcgen05" or (tensor_cores == "auto" and d == 128):
-        call(
-            "gk_attention_prefill_tc_tokens_bf16", ptr(q), ptr(kv.k), ptr(kv.v), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots),
-            ptr(kv.block_table), n_seqs, int(max_q_len), n_q, n_kv, d, kv.max_pages, kv.page_size, kv.k.shape[0],
-            float(scale), int(window), ptr(error_flag(q.device)), stream_ptr(), int(q.shape[0]), int(sink),
-        )
-        return out
-    call(
-        "gk_attention_prefill_bf16", ptr(q), ptr(kv.k), ptr(kv.v), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots),
-        ptr(kv.block_table), n_seqs, int(max_q_len), n_q, n_kv, d, kv.max_pages, kv.page_size, float(scale), int(window),
-        int(sink), stream_ptr(),
-    )
+    _launch_prefill(tensor_cores == "tcgen05" or (tensor_cores == "auto" and d == 128), q, ptr(kv.k), ptr(kv.v), kv.k.shape, out, ptr(cu_q), ptr(kv_len),
+                    ptr(slots), ptr(kv.block_table), n_seqs, kv.max_pages, int(max_q_len), float(scale), int(window), int(sink), ptr(error_flag(q.device)))
     return out
+
+
+def _launch_prefill(tcgen05: bool, q: torch.Tensor, k: int, v: int, sizes: tuple, out: torch.Tensor, cu_q: int, kv_len: int, slots: int, table: int, n_seqs: int,
+                    max_pages: int, max_q_len: int, scale: float, window: int, sink: int, error: int) -> None:
+    """``attention_prefill`` behind its checks, from addresses; ``sizes`` of the pages."""
+    n, n_q, d = q.shape
+    n_pages, n_kv, page, _ = sizes
+    if tcgen05:
+        call("gk_attention_prefill_tc_tokens_bf16", ptr(q), k, v, ptr(out), cu_q, kv_len, slots, table, n_seqs, max_q_len, n_q, n_kv, d, max_pages, page,
+             n_pages, scale, window, error, stream_ptr(), n, sink)
+    else:
+        call("gk_attention_prefill_bf16", ptr(q), k, v, ptr(out), cu_q, kv_len, slots, table, n_seqs, max_q_len, n_q, n_kv, d, max_pages, page, scale, window,
+             sink, stream_ptr())
 
 
 def set_attention_prefill_keys(keys: int) -> int:
@@ -2740,23 +2743,31 @@ def rows8_wins(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, n_kv
 
 
 # The prefill kernels read lengths and slots, inputs of a step elsewhere, before they wait for the kernel in front, which here is the one that writes them.
-_attention_prefill_in_order = in_order(attention_prefill)
+_launch_prefill_in_order = in_order(_launch_prefill)
 
 
-def _clean_pages8(kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, n_tokens: int, max_kv_len: int,
-                  last: int) -> tuple[PagedKV, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """The step's pages as bfloat16 with a table, starts, lengths and slots of their own.  Where the sequences could have more pages than there
-    are, pages keep their numbers."""
+def _prefill_clean8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, max_kv_len: int, scale: float,
+                    window: int, sink: bool, out: torch.Tensor) -> torch.Tensor:
+    """Prefill attention over the step's pages made bfloat16, with a table, starts, lengths and slots of their own.  Where the sequences could have more
+    pages than there are, pages keep their numbers.  (Two buffers and their addresses: as tensors of their own the host took longer over a
+    prompt of 2,048 tokens than the device.)"""
     n, device = kv_len.shape[0], kv.k.device
-    per = min(max(1, -(-int(max_kv_len) // kv.page_size)), kv.max_pages)
-    own_numbers = n * per > kv.k.shape[0]
-    shape = (kv.k.shape[0] if own_numbers else n * per, *kv.k.shape[1:])
-    k, v = (torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(2))
-    table, lens, own_slots, starts = torch.empty((n * per + 3 * n + 1,), dtype=torch.int32, device=device).split([n * per, n, n, n + 1])
-    table = table.view(n, per)
-    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), n_tokens, n, per, int(own_numbers), int(last), ptr(k), ptr(v), ptr(table), ptr(lens),
-         ptr(own_slots), ptr(starts), stream_ptr())
-    return PagedKV(k, v, table), starts, lens, own_slots
+    n_pages, n_kv, page, d = kv._sizes
+    per = min(max(1, -(-int(max_kv_len) // page)), kv._pages.max_pages)
+    own_numbers = n * per > n_pages
+    if not own_numbers:
+        n_pages = n * per
+    both = torch.empty((2, n_pages, n_kv, page, d), dtype=torch.bfloat16, device=device)
+    k = both.data_ptr()
+    v = k + 2 * n_pages * n_kv * page * d
+    ints = torch.empty((n * per + 3 * n + 1,), dtype=torch.int32, device=device)
+    table = ints.data_ptr()
+    lens, own_slots, starts = (table + 4 * n * (per + i) for i in range(3))
+    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n, per, int(own_numbers), window + max_q_len if 0 < window < max_kv_len else 0,
+         k, v, table, lens, own_slots, starts, stream_ptr())
+    _launch_prefill_in_order(d == 128, q, k, v, (n_pages, n_kv, page, d), out, starts, lens, own_slots, table, n, per, int(max_q_len), float(scale), int(window),
+                             int(sink), kv._pages.error)
+    return out
 
 
 def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: torch.Tensor, slots: torch.Tensor, max_q_len: int, max_kv_len: int,
@@ -2774,8 +2785,7 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and group <= ROWS8_MAX_GROUP and n_seqs and n_tokens:
         if rows8_wins(n_tokens, n_seqs, max_q_len, min(max_kv_len, window + max_q_len) if window else max_kv_len, n_kv, group, d, _sm_count_of(kv._index)):
             return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
-        pages, starts, lens, own_slots = _clean_pages8(kv, cu_q, kv_len, slots, n_tokens, max_kv_len, window + max_q_len if 0 < window < max_kv_len else 0)
-        return _attention_prefill_in_order(q, pages, starts, lens, own_slots, max_q_len, scale, window, out, sink=sink)
+        return _prefill_clean8(q, kv, cu_q, kv_len, slots, max_q_len, max_kv_len, scale, window, sink, out)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
          int(window), int(sink), stream_ptr())
     return out
