@@ -151,8 +151,8 @@ __global__ void __launch_bounds__(PF_WARPS * 32) attention_prefill_kernel(
     for (int h = 0; h < 2; ++h) {
         if (!row_ok[h]) continue;
         const int r = wrow0 + (lane >> 2) + 8 * h;
-        // with a sink the denominator has one more term: a key of score 0 that has no value
-        const float inv = 1.0f / (sink ? l[h] + exp2_fast(-m[h]) : l[h]);
+        // with a sink the denominator has one more term: a key of score 0 that has no value; a row that sees no key is zeros
+        const float sum = sink ? l[h] + exp2_fast(-m[h]) : l[h], inv = sum == 0.f ? 0.f : 1.0f / sum;
         __nv_bfloat16* orow = out + ((size_t)(q_begin + tok[h]) * n_q + (size_t)hk * group + (r % group)) * D;
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)

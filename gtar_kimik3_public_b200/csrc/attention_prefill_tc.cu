@@ -221,6 +221,10 @@ __global__ void __launch_bounds__(THREADS, 2) attention_prefill_tc_kernel(const 
     const int* pages = p.block_table + (size_t)p.slots[seq] * p.max_pages;
     const int last_row = min(row0 + ROWS, n_rows) - 1;
     const int max_pos = past + last_row / group, min_pos = past + row0 / group;
+    if (max_pos < 0) {  // more tokens than positions: none of these sees a key, and there is no page to load
+        pdl_wait();     // (who waits for this launch counts on its having waited)
+        return;
+    }
     const int lo_block = (p.window > 0 && min_pos - p.window + 1 > 0) ? min_pos - p.window + 1 : 0;
     const int p_begin = lo_block / PAGE, p_end = max_pos / PAGE + 1;
     const int n_iter = p_end - p_begin;
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_prefill_tc_kernel(const 
         if (ok && n_iter > 0) ok = mbar_wait(&sm.o_done, (n_iter - 1) & 1);
         fence_after();
         if (ok && n_iter > 0) {
-            const float inv = 1.0f / (p.sink ? l + exp2f(-m_used) : l);
+            const float sum = p.sink ? l + exp2f(-m_used) : l, inv = sum == 0.f ? 0.f : 1.0f / sum;  // (a row that sees no key: zeros)
             __nv_bfloat16* orow = p.out + ((size_t)(q_begin + tok) * p.n_q + head) * D;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -510,8 +514,14 @@ __global__ void __launch_bounds__(THREADS2, 1) attention_prefill_tc2_kernel(cons
     if ((p.one_tile ? first : 2 * first) >= n_blocks) return;  // whole block, before any barrier or allocation
     // the block's query tiles: the heavy one first
     const int tile_of[2] = {n_blocks - 1 - first, p.one_tile ? -1 : first};
-    const int n_tiles = tile_of[0] > tile_of[1] && !p.one_tile ? 2 : 1;
     const int len = p.kv_len[seq], past = len - q_len;
+    // with more tokens than positions, a tile none of whose tokens sees a key has no pages and is passed over
+    auto sees = [&](int tile) { return past >= 0 || past + over_group(min((tile + 1) * ROWS, n_rows) - 1) >= 0; };
+    if (!sees(tile_of[0])) {
+        pdl_wait();  // (who waits for this launch counts on its having waited)
+        return;
+    }
+    const int n_tiles = tile_of[0] > tile_of[1] && !p.one_tile && sees(tile_of[1]) ? 2 : 1;
     const int* pages = p.block_table + (size_t)p.slots[seq] * p.max_pages;
     // pages [p_begin, p_end) of query tile u, in steps of two
     auto span = [&](int u, int& p_begin, int& p_end) {
@@ -828,7 +838,7 @@ __global__ void __launch_bounds__(THREADS2, 1) attention_prefill_tc2_kernel(cons
             if (!ok) break;
             fence_after();
             // (with a sink: its term against the reference exponent, which both halves of a row share)
-            const float inv = 1.0f / (sm.row_sum[0][r] + sm.row_sum[1][r] + (p.sink ? exp2f(-m_used) : 0.f));
+            const float sum = sm.row_sum[0][r] + sm.row_sum[1][r] + (p.sink ? exp2f(-m_used) : 0.f), inv = sum == 0.f ? 0.f : 1.0f / sum;  // (sees no key: zeros)
             uint32_t packed[32];  // this thread's 64 columns of its row, then 16 columns of each row of the quad
 #pragma unroll
             for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -895,7 +905,7 @@ struct Tile {
     int p_begin, p_end;        // its pages, taken in steps of two
 };
 
-// Entry `item` of the launch's list; false if the sequence has no such tile.
+// Entry `item` of the launch's list; false if the sequence has no such tile, or one of no pages.
 __device__ __forceinline__ bool tile_of_item(const Params& p, int item, int group, Tile& t) {
     const int per = p.n_kv * p.n_seqs;
     const int from_end = item / per, rem = item - from_end * per;
@@ -911,6 +921,7 @@ __device__ __forceinline__ bool tile_of_item(const Params& p, int item, int grou
     t.pages = p.block_table + (size_t)p.slots[t.seq] * p.max_pages;
     const int row0 = t.tile * ROWS, last_row = min(row0 + ROWS, t.n_rows) - 1;
     const int max_pos = t.past + last_row / group, min_pos = t.past + row0 / group;
+    if (max_pos < 0) return false;  // more tokens than positions: none of these sees a key
     const int lo = (p.window > 0 && min_pos - p.window + 1 > 0) ? min_pos - p.window + 1 : 0;
     t.p_begin = lo / PAGE;
     t.p_end = max_pos / PAGE + 1;
@@ -1205,7 +1216,7 @@ __global__ void __launch_bounds__(THREADS2, 1) attention_prefill_tc5_kernel(cons
             if (!ok) break;
             fence_after();
             // (with a sink: its term against the reference exponent, which both halves of a row share)
-            const float inv = 1.0f / (sm.row_sum[0][r] + sm.row_sum[1][r] + (p.sink ? exp2f(-m_used) : 0.f));
+            const float sum = sm.row_sum[0][r] + sm.row_sum[1][r] + (p.sink ? exp2f(-m_used) : 0.f), inv = sum == 0.f ? 0.f : 1.0f / sum;  // (sees no key: zeros)
             uint32_t packed[32];
 #pragma unroll
             for (int c0 = 0; c0 < 64; c0 += 32) {

@@ -326,6 +326,8 @@ struct Clean8 {
     int *table, *kv_len, *slots, *cu_q;  // [n_seqs][per], [n_seqs], [n_seqs], [n_seqs + 1]
     const int* cu_q_in;
     int n_tokens, per, own_numbers;  // pages a sequence; whether a page keeps its number or is seq * per + index
+    __nv_bfloat16* out;              // [n_tokens][row]: attention's result; zeros here for tokens in front of their sequence's first position
+    int row;
 };
 
 // N numbers of a row as bfloat16: e4m3 times a power of two, exact.
@@ -348,7 +350,15 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
     pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.y, index = blockIdx.x, hk = blockIdx.z, d = HD ? HD : p.head_dim;
-    int len = length_of(p, kv_len[seq]);
+    const auto length_here = [&](int given) {
+        int len = length_of(p, given);
+        if (CLEAN && len > (long long)clean.per * p.page_size) {
+            if (p.error) *p.error = ERR_PLACE;
+            len = clean.per * p.page_size;
+        }
+        return len;
+    };
+    const int len = length_here(kv_len[seq]);
     if (CLEAN && seq == 0 && index == 0 && hk == 0 && threadIdx.x < 32) {  // starts within the queries, none before the one in front
         int before = 0;
         for (int base = 0; base <= (int)gridDim.y; base += 32) {
@@ -363,12 +373,19 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
                 clean.cu_q[i] = at;
                 if (at != given && p.error) *p.error = ERR_PLACE;
             }
+            // A sequence with more tokens than positions: its first tokens would stand in front of position 0.  They see no key and get zeros here;
+            // the prefill kernels pass over a tile of none but such.
+            int first = __shfl_up_sync(0xffffffffu, at, 1), blind = 0;
+            if (threadIdx.x == 0) first = before;
+            if (i > 0 && i <= (int)gridDim.y) blind = max(0, at - first - length_here(kv_len[i - 1]));
+            if (blind > 0 && p.error) *p.error = ERR_PLACE;
+            for (unsigned left = __ballot_sync(0xffffffffu, blind > 0); left; left &= left - 1) {
+                const int who = __ffs(left) - 1;
+                const size_t from = (size_t)__shfl_sync(0xffffffffu, first, who) * clean.row, n = (size_t)__shfl_sync(0xffffffffu, blind, who) * clean.row;
+                for (size_t c = threadIdx.x; c < n; c += 32) clean.out[from + c] = __float2bfloat16_rn(0.f);
+            }
             before = __shfl_sync(0xffffffffu, at, 31);
         }
-    }
-    if (CLEAN && len > (long long)clean.per * p.page_size) {
-        if (p.error) *p.error = ERR_PLACE;
-        len = clean.per * p.page_size;
     }
     const bool seen = (long long)index * p.page_size < len && (last <= 0 || (index + 1) * (long long)p.page_size > (long long)len - last);
     const int page = seen ? page_of(p, slots[seq], index) : -1;
@@ -497,15 +514,17 @@ GK_EXPORT int gk_read8(const GkPages8* pages, const int* kv_len, const int* slot
 }
 
 // The same for attention over what is read: `per` pages a sequence under numbers seq * per + index (`own_numbers`: their own), and `table`
-// [n_seqs][per], `len_out` and `slots_out` [n_seqs] and `cu_out` [n_seqs + 1] to go with them.  Heads of 64 or 128.
-GK_EXPORT int gk_clean8(const GkPages8* pages, const int* cu_q, const int* kv_len, const int* slots, int n_tokens, int n_seqs, int per, int own_numbers,
-                        int last, void* k_out, void* v_out, int* table, int* len_out, int* slots_out, int* cu_out, void* stream) {
+// [n_seqs][per], `len_out` and `slots_out` [n_seqs] and `cu_out` [n_seqs + 1] to go with them.  Heads of 64 or 128.  `out` [n_tokens][n_q][head_dim], where
+// the attention's result will be: a sequence's first tokens, where it brings more than it has positions, get zeros (and are reported).
+GK_EXPORT int gk_clean8(const GkPages8* pages, const int* cu_q, const int* kv_len, const int* slots, int n_tokens, int n_seqs, int n_q, int per,
+                        int own_numbers, int last, void* k_out, void* v_out, void* out, int* table, int* len_out, int* slots_out, int* cu_out, void* stream) {
     const int status = cache8::check(pages, "clean8");
     if (status != GK_OK) return status;
-    GK_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && per > 0 && last >= 0 && (long long)n_seqs * per < 2147483647LL, "clean8: bad sizes n_seqs=%d per=%d last=%d",
-               n_seqs, per, last);
+    GK_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && n_q > 0 && per > 0 && last >= 0 && (long long)n_seqs * per < 2147483647LL,
+               "clean8: bad sizes n_seqs=%d n_q=%d per=%d last=%d", n_seqs, n_q, per, last);
     if (n_seqs == 0) return GK_OK;
-    GK_REQUIRE(cu_q && kv_len && slots && k_out && v_out && table && len_out && slots_out && cu_out, "clean8: an array is missing");
+    GK_REQUIRE(cu_q && kv_len && slots && k_out && v_out && out && table && len_out && slots_out && cu_out, "clean8: an array is missing");
     return launch_read8<true>(*pages, kv_len, slots, n_seqs, per, last, k_out, v_out,
-                              Clean8{table, len_out, slots_out, cu_out, cu_q, n_tokens, per, own_numbers}, (cudaStream_t)stream);
+                              Clean8{table, len_out, slots_out, cu_out, cu_q, n_tokens, per, own_numbers, (__nv_bfloat16*)out, n_q * pages->head_dim},
+                              (cudaStream_t)stream);
 }

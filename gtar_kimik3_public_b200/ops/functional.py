@@ -2763,8 +2763,8 @@ def _prefill_clean8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: t
     ints = torch.empty((n * per + 3 * n + 1,), dtype=torch.int32, device=device)
     table = ints.data_ptr()
     lens, own_slots, starts = (table + 4 * n * (per + i) for i in range(3))
-    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n, per, int(own_numbers), window + max_q_len if 0 < window < max_kv_len else 0,
-         k, v, table, lens, own_slots, starts, stream_ptr())
+    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n, q.shape[1], per, int(own_numbers),
+         window + max_q_len if 0 < window < max_kv_len else 0, k, v, ptr(out), table, lens, own_slots, starts, stream_ptr())
     _launch_prefill_in_order(d == 128, q, k, v, (n_pages, n_kv, page, d), out, starts, lens, own_slots, table, n, per, int(max_q_len), float(scale), int(window),
                              int(sink), kv._pages.error)
     return out

@@ -1,0 +1,83 @@
+"""Several tokens a sequence over 8-bit pages where a sequence's numbers cannot be: fewer positions than tokens, none, a length below zero or beyond the
+bound.  Reported; tokens in front of the first position see no key and are zeros, the others and the step's other sequences are what they are."""
+
+import pytest
+import torch
+
+from tests.test_gpu_cache8 import DEV, F, SEVERAL, check_attention, held, ints, rand, sequences
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def way(request, monkeypatch):
+    """Through the kernel for few rows, through clean pages, or through the kernel for any size."""
+    monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: request.param == "few")
+    return torch.float32 if request.param == "any" else torch.bfloat16
+
+
+@pytest.fixture
+def dealt(request):
+    """How the tcgen05 prefill kernels deal out their tiles: (blocks that stay, one tile a block, keys a step)."""
+    from gtar_kimik3_public_b200.ops.library import library
+
+    stay, one, keys = request.param
+    before = (library().gk_set_attention_prefill_stay(stay), library().gk_set_attention_prefill_one_tile(one), library().gk_set_attention_prefill_keys(keys))
+    yield
+    library().gk_set_attention_prefill_stay(before[0])
+    library().gk_set_attention_prefill_one_tile(before[1])
+    library().gk_set_attention_prefill_keys(before[2])
+
+
+def check_lengths(dtype, d, window, sink, new, lens, wrong, given, bound):
+    """Sequence ``wrong`` is given the length ``given``; the longest length is said to be ``bound``."""
+    n_q, n_kv = 4, 2
+    kv, slots, table = sequences(lens, n_kv, d)
+    cu = [0]
+    for m in new:
+        cu.append(cu[-1] + m)
+    q = rand(cu[-1], n_q, d, seed=5).to(dtype)
+    said = list(lens)
+    said[wrong] = given
+    f = F()
+    good = f.attention_prefill8(q.to(DEV), kv, ints(*cu), ints(*lens), slots, max(new), max(lens), d**-0.5, window, sink)
+    f.check_kernel_errors(DEV)
+    out = torch.full(q.shape, 5.0, dtype=dtype, device=DEV)
+    f.attention_prefill8(q.to(DEV), kv, ints(*cu), ints(*said), slots, max(new), bound, d**-0.5, window, sink, out)
+    with pytest.raises(f.KernelError, match="length"):
+        f.check_kernel_errors(DEV)
+    for i in range(len(new)):
+        here = slice(cu[i], cu[i + 1])
+        if i != wrong:
+            assert torch.equal(out[here], good[here]), f"sequence {i}"
+            continue
+        length = max(0, min(given, -(-bound // 64) * 64))
+        blind = max(0, new[i] - length)
+        assert (out[here][:blind] == 0).all(), "tokens in front of position 0"
+        if blind < new[i]:
+            k, v = held(kv, table, int(slots[i]), lens[i])
+            check_attention(out[here][blind:], q[here][blind:], k[:length], v[:length], length - (new[i] - blind), window, sink, SEVERAL[dtype], "the rest")
+
+
+# new tokens, true lengths, which is wrong, what it is said to be, the bound on lengths
+WRONG = [([70, 1, 40], [200, 64, 40], 0, 0, 200),      # no positions, 70 tokens
+         ([70, 1, 40], [200, 64, 40], 0, -7, 200),     # less than none
+         ([70, 1, 40], [200, 64, 40], 0, 33, 200),     # tokens in front of position 0 and behind it in one tile
+         ([300, 5], [300, 90], 0, 100, 300),           # whole tiles in front of position 0
+         ([5, 300], [90, 300], 1, 1, 300),
+         ([300, 5], [300, 60], 0, 300, 64)]            # a bound that is too small
+
+
+@pytest.mark.parametrize("way", ["clean"], indirect=True)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sink", [(0, False), (40, True)])
+@pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG)
+def test_fewer_positions_than_tokens(way, d, window, sink, new, lens, wrong, given, bound):
+    check_lengths(way, d, window, sink, new, lens, wrong, given, bound)
+
+
+@pytest.mark.parametrize("way", ["clean"], indirect=True)
+@pytest.mark.parametrize("dealt", [(1, 1, 128), (0, 1, 128), (0, 0, 128), (0, 0, 64)], indirect=True)
+@pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG)
+def test_fewer_positions_than_tokens_in_every_prefill_kernel(way, dealt, new, lens, wrong, given, bound):
+    check_lengths(way, 128, 0, False, new, lens, wrong, given, bound)
