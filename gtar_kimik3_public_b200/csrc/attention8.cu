@@ -3,8 +3,8 @@
 // For a token at position pos of its sequence, query head hq, kv head hk = hq / (n_q / n_kv), visible keys j <= pos (and j > pos - window
 // where a window is set; src/layers/attention.py:116-119, src/ops/flash_attention_2.py:33-34):
 //   s_j = scale * (q . k8_j) * 2^ek_j        o = sum_j exp(s_j - m) 2^ev_j v8_j / sum_j exp(s_j - m),   m = max_j s_j
-// With `sink` one more term in the denominator: a key of score 0 without a value.  A token that sees no key gets zeros.  Keys that are
-// not visible are not looked at, whatever their places hold.
+// With `sink` one more term in the denominator: a key of score 0 without a value.  A token that sees no key gets zeros (one in front of position 0, of a
+// sequence that brings more tokens than it has positions, is reported as well).  Keys that are not visible are not looked at, whatever their places hold.
 
 #include "cache8.cuh"
 
@@ -50,6 +50,7 @@ __global__ void __launch_bounds__(128) attend8_rows_kernel(const GkPages8 p, con
         seq = sequence_of(a.cu_q, a.n_seqs, t);
         if (seq < 0) return;
         pos = length_of(p, a.kv_len[seq]) - a.cu_q[seq + 1] + t;
+        if (pos < 0 && p.error) *p.error = ERR_PLACE;  // more tokens than positions
     } else {
         pos = length_of(p, a.kv_len[seq]) - 1;
     }

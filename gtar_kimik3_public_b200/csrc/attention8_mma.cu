@@ -75,6 +75,7 @@ __device__ __forceinline__ Unit unit_of(const GkPages8& p, const Rows8& a, int u
             if (p.error) *p.error = ERR_PLACE;
             q_len = max(0, min(q_len, most));
         }
+        if (q_len > len && p.error) *p.error = ERR_PLACE;  // the first of them stand in front of position 0: they see no key
     }
     u.n_rows = min(most_rows, q_len * a.group - u.row_first);
     u.past = len - q_len;

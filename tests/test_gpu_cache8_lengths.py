@@ -81,3 +81,11 @@ def test_fewer_positions_than_tokens(way, d, window, sink, new, lens, wrong, giv
 @pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG)
 def test_fewer_positions_than_tokens_in_every_prefill_kernel(way, dealt, new, lens, wrong, given, bound):
     check_lengths(way, 128, 0, False, new, lens, wrong, given, bound)
+
+
+@pytest.mark.parametrize("way", ["few", "any"], indirect=True)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sink", [(0, False), (40, True)])
+@pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG[:-1])  # (a bound is no more than a hint to these kernels)
+def test_fewer_positions_than_tokens_without_clean_pages(way, d, window, sink, new, lens, wrong, given, bound):
+    check_lengths(way, d, window, sink, new, lens, wrong, given, bound)
