@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(128) attend8_rows_kernel(const GkPages8 p, con
     float m = -INFINITY, l = 0.f, acc[MAX_ACC];
 #pragma unroll
     for (int i = 0; i < MAX_ACC; ++i) acc[i] = 0.f;
-    const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+    const int lo = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;  // (the difference alone could leave 32 bits)
     for (int j0 = lo & ~31; j0 <= pos; j0 += 32) {  // a page is whole blocks of 32 keys
         const int page = page_of(p, slot, j0 / p.page_size), j = j0 + lane;
         if (page < 0) continue;  // its keys count as not visible

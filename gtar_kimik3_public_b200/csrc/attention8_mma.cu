@@ -81,9 +81,10 @@ __device__ __forceinline__ Unit unit_of(const GkPages8& p, const Rows8& a, int u
     u.past = len - q_len;
     u.pos_low = u.past + u.row_first / a.group;  // of the first row
     const int pos_high = u.past + (u.row_first + u.n_rows - 1) / a.group;
-    u.begin = a.window > 0 ? max(0, u.pos_low - a.window + 1) : 0;
+    // (compared first: a position in front of 0 less the largest window would leave 32 bits)
+    u.begin = a.window > 0 && u.pos_low >= a.window ? u.pos_low - a.window + 1 : 0;
     u.end = max(u.begin, pos_high + 1);
-    u.all_begin = a.window > 0 ? max(0, pos_high - a.window + 1) : 0;  // keys all_begin .. pos_low are seen by every row
+    u.all_begin = a.window > 0 && pos_high >= a.window ? pos_high - a.window + 1 : 0;  // keys all_begin .. pos_low are seen by every row
     u.tile_0 = u.begin / KEYS;
     u.n_tiles = u.n_rows > 0 ? (u.end + KEYS - 1) / KEYS - u.tile_0 : 0;
     return u;

@@ -75,18 +75,19 @@ __global__ void __launch_bounds__(PF_WARPS * 32) attention_prefill_kernel(
             }
         }
     }
-    // key range of the block: from the first key its first row may see to the last key its last row sees
+    // key range of the block: from the first key its first row may see to the last key its last row sees (positions and the window are compared before
+    // they are taken from each other: with more tokens than positions the first lie in front of 0, and less the largest window would leave 32 bits)
     const int last_row = min(row0 + PF_ROWS, n_rows) - 1;
     const int max_pos = past + last_row / group;
     const int min_pos = past + row0 / group;
-    const int lo_block = (window > 0 && min_pos - window + 1 > 0) ? min_pos - window + 1 : 0;
+    const int lo_block = window > 0 && min_pos >= window ? min_pos - window + 1 : 0;
     const int p_begin = lo_block / PAGE, p_end = max_pos / PAGE + 1;
     const int n_iter = p_end - p_begin;
     // of this warp
     const int w_last_row = min(wrow0 + 16, n_rows) - 1;
     const int w_max_pos = w_last_row >= wrow0 ? past + w_last_row / group : -1;
     const int w_min_pos = past + wrow0 / group;
-    const int w_lo = (window > 0 && w_min_pos - window + 1 > 0) ? w_min_pos - window + 1 : 0;
+    const int w_lo = window > 0 && w_min_pos >= window ? w_min_pos - window + 1 : 0;
 
     auto issue = [&](int it) {
         if (it < n_iter) {

@@ -197,7 +197,7 @@ struct Params {
     const int* block_table;
     int n_q, n_kv, max_pages;
     float sl2;
-    int window;
+    int window;  // (compared with a position before it is taken from it: one in front of 0 less the largest window would leave 32 bits)
     int sink;  // one more term in the softmax's denominator: a key of score 0 that has no value
     int* error_flag;
     int one_tile;  // tc2: a query tile a block, heaviest first (grid: kv head, sequence, tile), instead of a heavy and a light one
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_prefill_tc_kernel(const 
         pdl_wait();     // (who waits for this launch counts on its having waited)
         return;
     }
-    const int lo_block = (p.window > 0 && min_pos - p.window + 1 > 0) ? min_pos - p.window + 1 : 0;
+    const int lo_block = p.window > 0 && min_pos >= p.window ? min_pos - p.window + 1 : 0;
     const int p_begin = lo_block / PAGE, p_end = max_pos / PAGE + 1;
     const int n_iter = p_end - p_begin;
 
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(THREADS2, 1) attention_prefill_tc2_kernel(cons
         const int row0 = tile_of[u] * ROWS;
         const int last_row = min(row0 + ROWS, n_rows) - 1;
         const int max_pos = past + over_group(last_row), min_pos = past + over_group(row0);
-        const int lo = (p.window > 0 && min_pos - p.window + 1 > 0) ? min_pos - p.window + 1 : 0;
+        const int lo = p.window > 0 && min_pos >= p.window ? min_pos - p.window + 1 : 0;
         p_begin = lo / PAGE;
         p_end = max_pos / PAGE + 1;
     };
@@ -922,7 +922,7 @@ __device__ __forceinline__ bool tile_of_item(const Params& p, int item, int grou
     const int row0 = t.tile * ROWS, last_row = min(row0 + ROWS, t.n_rows) - 1;
     const int max_pos = t.past + last_row / group, min_pos = t.past + row0 / group;
     if (max_pos < 0) return false;  // more tokens than positions: none of these sees a key
-    const int lo = (p.window > 0 && min_pos - p.window + 1 > 0) ? min_pos - p.window + 1 : 0;
+    const int lo = p.window > 0 && min_pos >= p.window ? min_pos - p.window + 1 : 0;
     t.p_begin = lo / PAGE;
     t.p_end = max_pos / PAGE + 1;
     return true;

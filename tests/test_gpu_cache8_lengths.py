@@ -89,3 +89,21 @@ def test_fewer_positions_than_tokens_in_every_prefill_kernel(way, dealt, new, le
 @pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG[:-1])  # (a bound is no more than a hint to these kernels)
 def test_fewer_positions_than_tokens_without_clean_pages(way, d, window, sink, new, lens, wrong, given, bound):
     check_lengths(way, d, window, sink, new, lens, wrong, given, bound)
+
+
+@pytest.mark.parametrize("way", ["few", "clean", "any"], indirect=True)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cut", [(2, 0), (0, 40)])
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 40])
+@pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG[:-1])
+def test_the_largest_windows_in_front_of_position_0(way, d, cut, window, new, lens, wrong, given, bound, monkeypatch):
+    """A position below zero less the largest window would leave 32 bits: as if there were no window."""
+    monkeypatch.setattr(F(), "rows8_cut", lambda *sizes: cut)
+    check_lengths(way, d, window, False, new, lens, wrong, given, bound)
+
+
+@pytest.mark.parametrize("way", ["clean"], indirect=True)
+@pytest.mark.parametrize("dealt", [(1, 1, 128), (0, 1, 128), (0, 0, 128), (0, 0, 64)], indirect=True)
+@pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG)
+def test_the_largest_window_in_every_prefill_kernel(way, dealt, new, lens, wrong, given, bound):
+    check_lengths(way, 128, 2**31 - 1, False, new, lens, wrong, given, bound)
