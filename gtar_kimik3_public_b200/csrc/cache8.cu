@@ -326,7 +326,8 @@ struct Clean8 {
     int *table, *kv_len, *slots, *cu_q;  // [n_seqs][per], [n_seqs], [n_seqs], [n_seqs + 1]
     const int* cu_q_in;
     int n_tokens, per, own_numbers;  // pages a sequence; whether a page keeps its number or is seq * per + index
-    __nv_bfloat16* out;              // [n_tokens][row]: attention's result; zeros here for tokens in front of their sequence's first position
+    int max_q_len, window;           // what the attention is launched for: tokens a sequence at most, keys a token sees (0: all)
+    __nv_bfloat16* out;              // [n_tokens][row]: its result; zeros here for tokens in front of their sequence's first position
     int row;
 };
 
@@ -373,12 +374,12 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
                 clean.cu_q[i] = at;
                 if (at != given && p.error) *p.error = ERR_PLACE;
             }
-            // A sequence with more tokens than positions: its first tokens would stand in front of position 0.  They see no key and get zeros here;
+            // A sequence with more tokens than the attention is launched for: the rest of them is left out.  With more tokens than positions: its first tokens would stand in front of position 0.  They see no key and get zeros here;
             // the prefill kernels pass over a tile of none but such.
             int first = __shfl_up_sync(0xffffffffu, at, 1), blind = 0;
             if (threadIdx.x == 0) first = before;
             if (i > 0 && i <= (int)gridDim.y) blind = max(0, at - first - length_here(kv_len[i - 1]));
-            if (blind > 0 && p.error) *p.error = ERR_PLACE;
+            if ((blind > 0 || (i > 0 && at - first > clean.max_q_len)) && p.error) *p.error = ERR_PLACE;
             for (unsigned left = __ballot_sync(0xffffffffu, blind > 0); left; left &= left - 1) {
                 const int who = __ffs(left) - 1;
                 const size_t from = (size_t)__shfl_sync(0xffffffffu, first, who) * clean.row, n = (size_t)__shfl_sync(0xffffffffu, blind, who) * clean.row;
@@ -387,7 +388,12 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
             before = __shfl_sync(0xffffffffu, at, 31);
         }
     }
-    const bool seen = (long long)index * p.page_size < len && (last <= 0 || (index + 1) * (long long)p.page_size > (long long)len - last);
+    long long back = last;  // how many of the sequence's last positions are wanted (0: all)
+    if (CLEAN && clean.window > 0) {  // those that its first token sees, and on; starts that are put in order make no sequence longer
+        const int from = max(clean.cu_q_in[seq], 0), to = min(clean.cu_q_in[seq + 1], clean.n_tokens);
+        back = (long long)clean.window + max(0, to - from);
+    }
+    const bool seen = (long long)index * p.page_size < len && (back <= 0 || (index + 1) * (long long)p.page_size > (long long)len - back);
     const int page = seen ? page_of(p, slots[seq], index) : -1;
     int to_page = page;
     if (CLEAN) {
@@ -514,17 +520,18 @@ GK_EXPORT int gk_read8(const GkPages8* pages, const int* kv_len, const int* slot
 }
 
 // The same for attention over what is read: `per` pages a sequence under numbers seq * per + index (`own_numbers`: their own), and `table`
-// [n_seqs][per], `len_out` and `slots_out` [n_seqs] and `cu_out` [n_seqs + 1] to go with them.  Heads of 64 or 128.  `out` [n_tokens][n_q][head_dim], where
-// the attention's result will be: a sequence's first tokens, where it brings more than it has positions, get zeros (and are reported).
+// [n_seqs][per], `len_out` and `slots_out` [n_seqs] and `cu_out` [n_seqs + 1] to go with them.  Heads of 64 or 128.  `window`: pages
+// that no token sees are left out (0: none are).  `out` [n_tokens][n_q][head_dim], where the attention's result will be: a sequence's first tokens, where
+// it brings more than it has positions, get zeros.  That is reported, and so are more tokens than `max_q_len`.
 GK_EXPORT int gk_clean8(const GkPages8* pages, const int* cu_q, const int* kv_len, const int* slots, int n_tokens, int n_seqs, int n_q, int per,
-                        int own_numbers, int last, void* k_out, void* v_out, void* out, int* table, int* len_out, int* slots_out, int* cu_out, void* stream) {
+                        int own_numbers, int max_q_len, int window, void* k_out, void* v_out, void* out, int* table, int* len_out, int* slots_out, int* cu_out,
+                        void* stream) {
     const int status = cache8::check(pages, "clean8");
     if (status != GK_OK) return status;
-    GK_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && n_q > 0 && per > 0 && last >= 0 && (long long)n_seqs * per < 2147483647LL,
-               "clean8: bad sizes n_seqs=%d n_q=%d per=%d last=%d", n_seqs, n_q, per, last);
+    GK_REQUIRE(n_seqs >= 0 && n_seqs <= 65535 && n_q > 0 && per > 0 && max_q_len >= 0 && window >= 0 && (long long)n_seqs * per < 2147483647LL,
+               "clean8: bad sizes n_seqs=%d n_q=%d per=%d max_q_len=%d window=%d", n_seqs, n_q, per, max_q_len, window);
     if (n_seqs == 0) return GK_OK;
     GK_REQUIRE(cu_q && kv_len && slots && k_out && v_out && out && table && len_out && slots_out && cu_out, "clean8: an array is missing");
-    return launch_read8<true>(*pages, kv_len, slots, n_seqs, per, last, k_out, v_out,
-                              Clean8{table, len_out, slots_out, cu_out, cu_q, n_tokens, per, own_numbers, (__nv_bfloat16*)out, n_q * pages->head_dim},
-                              (cudaStream_t)stream);
+    const Clean8 clean = {table, len_out, slots_out, cu_out, cu_q, n_tokens, per, own_numbers, max_q_len, window, (__nv_bfloat16*)out, n_q * pages->head_dim};
+    return launch_read8<true>(*pages, kv_len, slots, n_seqs, per, 0, k_out, v_out, clean, (cudaStream_t)stream);
 }

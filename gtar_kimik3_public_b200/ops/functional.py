@@ -2763,8 +2763,8 @@ def _prefill_clean8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len: t
     ints = torch.empty((n * per + 3 * n + 1,), dtype=torch.int32, device=device)
     table = ints.data_ptr()
     lens, own_slots, starts = (table + 4 * n * (per + i) for i in range(3))
-    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n, q.shape[1], per, int(own_numbers),
-         window + max_q_len if 0 < window < max_kv_len else 0, k, v, ptr(out), table, lens, own_slots, starts, stream_ptr())
+    call("gk_clean8", kv._at, ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n, q.shape[1], per, int(own_numbers), int(max_q_len),
+         int(window), k, v, ptr(out), table, lens, own_slots, starts, stream_ptr())
     _launch_prefill_in_order(d == 128, q, k, v, (n_pages, n_kv, page, d), out, starts, lens, own_slots, table, n, per, int(max_q_len), float(scale), int(window),
                              int(sink), kv._pages.error)
     return out
@@ -2774,7 +2774,8 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
                        scale: float, window: int = 0, sink: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the packed new tokens ``q [n_tokens, n_q, d]`` (bfloat16 or float32) over 8-bit pages.  Sequence ``i`` owns the tokens
     ``cu_q[i] .. cu_q[i+1]-1``, its last positions: ``kv_len[i]`` counts its cached tokens including them.  ``max_q_len`` and ``max_kv_len`` are the
-    largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were."""
+    largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were.  A sequence with more tokens than positions or than
+    ``max_q_len`` is reported; tokens in front of its first position get zeros."""
     out = _check_queries8(q, kv, out)
     n_seqs = kv_len.shape[0]
     if not (_fine8(kv, q, kv_len, slots, (n_seqs,)) and _fine8(kv, q, cu_q, cu_q, (n_seqs + 1,))):

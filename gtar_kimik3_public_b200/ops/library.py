@@ -117,7 +117,7 @@ _SIGNATURES: dict[str, list] = {
     "gk_rows8": [P, P, P, P, P, P, I, I, I, I, I, I, I, P, F, I, I, P],
     "gk_rows8_fused": [P, P, P, P, I, I, F, P, P, I, I, I, P, P, P, I, I, I, I, I, P, F, I, P],
     "gk_rows8_places": [I, I, I],
-    "gk_clean8": [P, P, P, P, I, I, I, I, I, I, P, P, P, P, P, P, P, P],
+    "gk_clean8": [P, P, P, P, I, I, I, I, I, I, I, P, P, P, P, P, P, P, P],
     "gk_attend8": [P, P, I, P, P, P, P, I, I, I, F, I, I, P],
     "gk_attention_scored_bf16": [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, P, P, P, I, I, I, P, P, I, P, F, L, F, P],
 }

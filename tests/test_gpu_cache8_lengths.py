@@ -107,3 +107,38 @@ def test_the_largest_windows_in_front_of_position_0(way, d, cut, window, new, le
 @pytest.mark.parametrize("new,lens,wrong,given,bound", WRONG)
 def test_the_largest_window_in_every_prefill_kernel(way, dealt, new, lens, wrong, given, bound):
     check_lengths(way, 128, 2**31 - 1, False, new, lens, wrong, given, bound)
+
+
+@pytest.mark.parametrize("way", ["few", "clean"], indirect=True)
+@pytest.mark.parametrize("d", [64, 128])
+def test_more_tokens_than_max_q_len(way, d):
+    """Reported whichever kernel takes them; the step's other sequences are what they are."""
+    kv, slots, _ = sequences([300, 90], 2, d)
+    q = rand(275, 4, d, seed=5).to(way).to(DEV)
+    args = (kv, ints(0, 270, 275), ints(300, 90), slots)
+    good = F().attention_prefill8(q, *args, 270, 300, d**-0.5)
+    F().check_kernel_errors(DEV)
+    for most in (0, 2, 100, 269):
+        got = F().attention_prefill8(q, *args, most, 300, d**-0.5)
+        with pytest.raises(F().KernelError, match="length"):
+            F().check_kernel_errors(DEV)
+        if most >= 5:
+            assert torch.equal(got[270:], good[270:])
+
+
+@pytest.mark.parametrize("way", ["clean"], indirect=True)
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_window_over_more_tokens_than_max_q_len(way, d):
+    """What the launch covers of such a sequence, its last tile, sees clean pages: the window goes back from the sequence's own first token."""
+    n_q, n_kv, new, n, window = 4, 2, 200, 271, 10
+    kv, slots, table = sequences([n], n_kv, d)
+    q = rand(new, n_q, d, seed=5).to(way)
+    # the memory that the call will take for its pages holds NaN
+    poison = torch.full((2, -(-n // 64), n_kv, 64, d), float("nan"), dtype=torch.bfloat16, device=DEV)
+    del poison
+    out = torch.full(q.shape, 5.0, dtype=way, device=DEV)
+    F().attention_prefill8(q.to(DEV), kv, ints(0, new), ints(n), slots, 2, n, d**-0.5, window, False, out)
+    with pytest.raises(F().KernelError, match="length"):
+        F().check_kernel_errors(DEV)
+    k, v = held(kv, table, int(slots[0]), n)
+    check_attention(out[-8:], q[-8:], k, v, n - 8, window, False, SEVERAL[way], "the last tokens")
