@@ -288,7 +288,8 @@ __device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, cons
     constexpr int E = D / 64, HALF = D / 2;
     const int pos = u.past;
     const __nv_bfloat16* row = f.qkv + ((size_t)u.first_token * (a.n_q + 2 * p.n_kv) + a.n_q + hk) * D;
-    if (f.cos_table != nullptr && (unsigned)pos >= (unsigned)f.table_positions && p.error) *p.error = ERR_PLACE;
+    const bool known = f.cos_table == nullptr || (unsigned)pos < (unsigned)f.table_positions;  // without a rotation the key stays out of the cache
+    if (!known && p.error) *p.error = ERR_PLACE;
     float x[2][2][E];
     int b[2];
 #pragma unroll
@@ -299,21 +300,22 @@ __device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, cons
     for (int v = 0; v < 2; ++v) {
         const float back = power_back(b[v]);
         uint8_t* to = (v ? p.v : p.k) + place * D;
+        const bool kept = page >= 0 && (v || known);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int at = h * HALF + lane * E;
             const uint32_t two = pack2(x[v][h][0] * back, x[v][h][E - 1] * back);
             if constexpr (E == 2) {
                 *reinterpret_cast<uint16_t*>(&bytes[v][at]) = (uint16_t)two;
-                if (page >= 0) *reinterpret_cast<uint16_t*>(to + at) = (uint16_t)two;
+                if (kept) *reinterpret_cast<uint16_t*>(to + at) = (uint16_t)two;
             } else {
                 bytes[v][at] = (unsigned char)two;
-                if (page >= 0) to[at] = (uint8_t)two;
+                if (kept) to[at] = (uint8_t)two;
             }
         }
         if (lane == 0) {
             powers[v] = (unsigned char)b[v];
-            if (page >= 0) (v ? p.v_exp : p.k_exp)[place] = (uint8_t)b[v];
+            if (kept) (v ? p.v_exp : p.k_exp)[place] = (uint8_t)b[v];
         }
     }
     __syncwarp();
