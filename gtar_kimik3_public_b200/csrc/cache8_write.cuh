@@ -137,6 +137,9 @@ __device__ __forceinline__ float to_be_rounded(float high, float low) {
     return __uint_as_float((__float_as_uint(h) - ((l < 0.f) != (h < 0.f) ? 1u : 0u)) | 1u);
 }
 
+constexpr float LARGE_SQUARES = 0x1p120f;
+constexpr float SMALL_MEAN = 0x1p-60f;  // below it the mean of squares and eps lose bits of squares that end at 2^-149
+
 // A key, or a row of values as it is, by LANES lanes that have HD / 2 / LANES neighbouring numbers of each half: the numbers to be rounded; the byte of the
 // row's power comes back.
 template <int HD, int LANES, typename TW>
@@ -151,21 +154,45 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
     }
     if (!is_v) {
         if (a.use_norm) {
-            Two8 ss = {0.f, 0.f};
+            const auto squares = [&] {
+                Two8 ss = {0.f, 0.f};
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < E; ++i) {  // (the square of a bfloat16 number is exact)
-                    const Two8 t = sum_of(ss.h, __fmul_rn(x[h][i], x[h][i]));
-                    ss = {t.h, __fadd_rn(ss.l, t.l)};
+                    for (int i = 0; i < E; ++i) {  // (the square of a bfloat16 number is exact, where it is one of 32 bits)
+                        const Two8 t = sum_of(ss.h, __fmul_rn(x[h][i], x[h][i]));
+                        ss = {t.h, __fadd_rn(ss.l, t.l)};
+                    }
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) {
+                    const float oh = __shfl_xor_sync(mask, ss.h, o), ol = __shfl_xor_sync(mask, ss.l, o);
+                    const Two8 t = sum_of(ss.h, oh);
+                    ss = {t.h, __fadd_rn(t.l, __fadd_rn(ss.l, ol))};
                 }
+                return ss;
+            };
+            Two8 ss = squares();
+            float eps = a.eps;
+            if (!(ss.h < LARGE_SQUARES) || (ss.h < SMALL_MEAN && eps < SMALL_MEAN)) {  // (the same for the lanes of the row)
+                // Squares that leave 32 bits: the row times a power of two, and eps times its square, come to the same.  The row's largest finite number
+                // becomes one of 1 to 2, or less where eps would leave 32 bits; what of eps is lost is nothing beside the squares then.
+                float top = 0.f;
 #pragma unroll
-            for (int o = 1; o < LANES; o <<= 1) {
-                const float oh = __shfl_xor_sync(mask, ss.h, o), ol = __shfl_xor_sync(mask, ss.l, o);
-                const Two8 t = sum_of(ss.h, oh);
-                ss = {t.h, __fadd_rn(t.l, __fadd_rn(ss.l, ol))};
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) top = fmaxf(top, finite_abs(x[h][i]));
+#pragma unroll
+                for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+                const int up = min(127 - (int)(__float_as_uint(top) >> 23), eps > 0.f ? 50 - ((int)(__float_as_uint(eps) >> 23) - 127) / 2 : 120);
+                const float half = __uint_as_float((uint32_t)(127 + up / 2) << 23), rest = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);  // 2^up in two factors
+                eps = ((eps * half) * half) * rest * rest;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) x[h][i] = (x[h][i] * half) * rest;
+                ss = squares();
             }
-            const Two8 m = sum_of(ss.h * (1.f / HD), a.eps);  // (HD is a power of two)
+            const Two8 m = sum_of(ss.h * (1.f / HD), eps);  // (HD is a power of two)
             const float ml = fmaf(ss.l, 1.f / HD, m.l);
             float r = rsqrtf(m.h), dr = 0.f;
             if (m.h < INFINITY && m.h > 0.f) {  // 1 / sqrt(m) = r + dr: a step of Newton's
@@ -229,16 +256,19 @@ __device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* r
     return b;
 }
 
-// RMSNorm and rotation of a row in 32 bits.
+// RMSNorm and rotation of a row in 32 bits.  Returns whether its mean of squares has lost bits at the range's lower end (one that leaves the upper end makes
+// the row zeros, which `make_bytes` sees).
 template <int HD>
-__device__ __forceinline__ void norm_rotate_32(const Norm8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16], const float (&w1)[HD / 16],
+__device__ __forceinline__ bool norm_rotate_32(const Norm8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16], const float (&w1)[HD / 16],
                                                const float (&c)[HD / 16], const float (&sn)[HD / 16], bool turns, unsigned mask) {
     constexpr int E = HD / 16;
+    bool lost = false;
     if (a.use_norm) {
         float ss = sum_of_squares(x, y);
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float inv = rsqrtf(fmaf(ss, 1.f / HD, a.eps));
+        const float mean = fmaf(ss, 1.f / HD, a.eps), inv = rsqrtf(mean);
+        lost = mean < SMALL_MEAN;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             x[i] = (x[i] * inv) * w0[i];
@@ -253,12 +283,14 @@ __device__ __forceinline__ void norm_rotate_32(const Norm8& a, float (&x)[HD / 1
             y[i] = v * c[i] + u * sn[i];
         }
     }
+    return lost;
 }
 
-// A lane's bytes of a key (normed and rotated in 32 bits, `row` what it was made of) or of a row of values; the byte of the row's power comes back.
+// A lane's bytes of a key (normed and rotated in 32 bits, `row` what it was made of, `lost` as above) or of a row of values; the byte of the row's power
+// comes back.
 template <int HD, typename TW>
-__device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 16], const float (&y)[HD / 16], bool turns, bool is_v, const __nv_bfloat16* row,
-                                          int pos, int sub, unsigned mask, uint32_t (&four)[2][HD / 64]) {
+__device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 16], const float (&y)[HD / 16], bool turns, bool is_v, bool lost,
+                                          const __nv_bfloat16* row, int pos, int sub, unsigned mask, uint32_t (&four)[2][HD / 64]) {
     constexpr int E = HD / 16;
     float top = 0.f;
 #pragma unroll
@@ -268,7 +300,7 @@ __device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 
     const int b = exponent_byte(top);
     const float back = power_back(b);
     // (a row that holds an infinity or NaN and is normed: its maximum is 0 or not to be trusted)
-    bool care = top == INFINITY || (!is_v && a.use_norm && top == 0.f);
+    bool care = top == INFINITY || lost || (!is_v && a.use_norm && top == 0.f);
     if (is_v || !(a.use_norm || turns)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)

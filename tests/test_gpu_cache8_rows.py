@@ -1,17 +1,78 @@
-"""Rows on their way into the 8-bit cache that are not ordinary ones, in every kernel that writes."""
+"""Rows on their way into the 8-bit cache that are not ordinary ones, in every kernel that writes: few tokens, many, any head size, and the decode kernel that
+writes its own token.  Each key is the formula in 64 bits rounded once."""
 
 import pytest
 import torch
 
+from tests.plain import cache8 as plain8
 from tests.plain import model as plain
 from tests.test_gpu_cache8 import DEV, F, empty_pages, held, ints, rand
 
 pytestmark = pytest.mark.gpu
 
+WAYS = ["few", "many", "decode"]
+
+
+def written(way, qkv, n_q, n_kv, d, eps, weight, cos, sin, positions):
+    """Keys and values ``[n, n_kv, d]`` as the cache holds them after the rows of ``qkv`` were written, one a sequence at ``positions``: by the write of few
+    tokens, by that of many (the same rows as often as it takes), or by the decode kernel."""
+    n = qkv.shape[0]
+    kv, slots, table = empty_pages(n, max(positions) + 1, n_kv, d)
+    table_args = [None if t is None else t.to(DEV) for t in (weight, weight, cos, sin)]
+    how = (*table_args[:2], eps, *table_args[2:])
+    if way == "decode":
+        for t in (kv.k, kv.v):  # places before the new one: zeros under some power
+            t.view(torch.uint8).zero_()
+        kv.k_exp.fill_(127)
+        kv.v_exp.fill_(127)
+        F().attention_decode8_fused(qkv.to(DEV), n_q, n_kv, d, *how, kv, ints(*[p + 1 for p in positions]), slots, max(positions), max(positions) + 1, 0.1)
+    else:
+        times = 1 if way == "few" else -(-(7 << 20) // (n * (n_q + 2 * n_kv) * d))
+        tokens = [i for _ in range(times) for i in range(n)]  # (the same row to the same place: whichever comes last)
+        F().qk_norm_rope_write8(qkv[tokens].to(DEV), n_q, n_kv, d, *how, ints(*[positions[i] for i in tokens]), ints(*tokens), slots, kv, max(positions))
+    F().check_kernel_errors(DEV)
+    rows = [held(kv, table, int(slots[i]), p + 1) for i, p in enumerate(positions)]
+    return [torch.stack([r[j][-1] for r in rows]) for j in (0, 1)]
+
+
+def formula(x, weight, eps, cos, sin, positions):
+    """RMSNorm and rotation of keys ``[n, n_kv, d]`` in 64 bits."""
+    x = x.double()
+    if weight is not None:
+        x = plain.rms_norm(x, weight.double(), eps)
+    if cos is not None:
+        c, s = (torch.cat([t, t], -1).double()[positions] for t in (cos, sin))
+        x = plain.apply_rotary(x, c, s)
+    return x
+
 
 def tables(positions, d):
     cos, sin = plain.rotary_tables(torch.arange(positions), d, 1e4)
     return cos[:, : d // 2].float().contiguous(), sin[:, : d // 2].float().contiguous()
+
+
+def equal(got, want, what):
+    want = plain8.quantised(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want)), what
+
+
+@pytest.mark.parametrize("way,d", [(w, d) for w in WAYS for d in (64, 128)] + [("few", 32), ("few", 80)])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_normed_rows_of_any_size(way, d, eps):
+    """Rows of 2^-110 to 2^126: their squares leave 32 bits on both sides, their norm does not."""
+    powers = [-110, -70, -64, -30, 0, 40, 62, 63, 64, 80, 100, 126]
+    n, n_q, n_kv = len(powers), 2, 2
+    keys = rand(n, n_kv, d, seed=1).clamp(-1.9, 1.9) * torch.tensor([2.0**p for p in powers], dtype=torch.float64).view(-1, 1, 1)
+    keys[5, 0, 1:] = 0  # one number alone
+    keys[7, 1, : d - 1] *= 2.0**-60  # and one far above the others
+    qkv = torch.cat([rand(n, n_q, d, seed=2), keys, rand(n, n_kv, d, seed=3)], 1).to(torch.bfloat16)
+    weight = (1 + 0.1 * rand(d, seed=4)).float()
+    positions = [3 * i for i in range(n)]
+    cos, sin = tables(40, d)
+    got, values = written(way, qkv.view(n, -1), n_q, n_kv, d, eps, weight, cos, sin, positions)
+    equal(got, formula(qkv[:, n_q:n_q + n_kv], weight, eps, cos, sin, positions), "keys")
+    equal(values, qkv[:, n_q + n_kv:].double(), "values")
 
 
 @pytest.mark.parametrize("n_q,n_kv,d", [(4, 2, 128), (6, 2, 64)])
