@@ -137,7 +137,7 @@ __device__ __forceinline__ float to_be_rounded(float high, float low) {
     return __uint_as_float((__float_as_uint(h) - ((l < 0.f) != (h < 0.f) ? 1u : 0u)) | 1u);
 }
 
-constexpr float LARGE_SQUARES = 0x1p120f;
+constexpr float LARGEST = 3.402823466e38f, LARGE_SQUARES = 0x1p120f;
 constexpr float SMALL_MEAN = 0x1p-60f;  // below it the mean of squares and eps lose bits of squares that end at 2^-149
 
 // A key, or a row of values as it is, by LANES lanes that have HD / 2 / LANES neighbouring numbers of each half: the numbers to be rounded; the byte of the
@@ -225,6 +225,10 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
                     const Two8 p = product_of(h ? v : u, c[i]), q = product_of(h ? u : v, s), t = sum_of(p.h, q.h);
                     x[h][i] = t.h;
                     low[h][i] = __fadd_rn(__fadd_rn(t.l, __fadd_rn(p.l, q.l)), __fmaf_rn(h ? vl : ul, c[i], __fmul_rn(h ? ul : vl, s)));
+                    if (fabsf(t.h) == INFINITY && fabsf(u) < INFINITY && fabsf(v) < INFINITY) {  // of finite numbers: the largest that there is
+                        x[h][i] = copysignf(LARGEST, t.h);
+                        low[h][i] = 0.f;
+                    }
                 }
             }
         }

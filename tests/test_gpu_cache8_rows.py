@@ -75,6 +75,21 @@ def test_normed_rows_of_any_size(way, d, eps):
     equal(values, qkv[:, n_q + n_kv:].double(), "values")
 
 
+@pytest.mark.parametrize("way,d", [(w, d) for w in WAYS for d in (64, 128)] + [("few", 32)])
+def test_rotated_rows_beyond_the_largest_number(way, d):
+    """Two numbers near the largest whose rotation mixes them to more than 32 bits hold: the largest number that the cache holds, as the formula's is."""
+    n, n_q, n_kv = 6, 2, 1
+    keys = torch.full((n, n_kv, d), 3.3e38, dtype=torch.float64)
+    keys[1::2, :, : d // 2] *= -1
+    qkv = torch.cat([rand(n, n_q, d, seed=2), keys, rand(n, n_kv, d, seed=3)], 1).to(torch.bfloat16)
+    positions = [0, 1, 2, 3, 4, 5]
+    cos, sin = tables(6, d)
+    got, _ = written(way, qkv.view(n, -1), n_q, n_kv, d, 1e-6, None, cos, sin, positions)
+    want = formula(qkv[:, n_q:n_q + n_kv], None, 0.0, cos, sin, positions)
+    assert (want.abs() > 3.5e38).any()
+    equal(got, want, "keys")
+
+
 @pytest.mark.parametrize("n_q,n_kv,d", [(4, 2, 128), (6, 2, 64)])
 def test_a_position_outside_the_rotation_s_table(n_q, n_kv, d):
     """The decode kernel leaves such a token's key where it was, writes its value and reports it, as the write by itself does; the others are what they are."""
