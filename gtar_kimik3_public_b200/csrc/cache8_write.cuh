@@ -312,9 +312,11 @@ __device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 
             for (int i = 0; i < E; i += 4)
                 four[h][i / 4] = pack2_finite((h ? y : x)[i] * back, (h ? y : x)[i + 1] * back) | pack2_finite((h ? y : x)[i + 2] * back, (h ? y : x)[i + 3] * back) << 16;
     } else {
-        // Off by 1.5 * 2^-21 of itself at most through the norm's factor, and by 2^-21 of both numbers that the rotation mixes through the roundings of
-        // their products: where as much less and as much more are not the same byte, or the maximum lies within 2^-18 of the next power's, the row
-        // is made over.
+        // How far a number x of a rotated pair (x, y) is from the formula, with r = 2^-24 for a rounding: 8 r of itself through the norm's factor (seven
+        // roundings of the sum of squares and one of the mean, halved by the root; rsqrtf's two steps, 4 r), 3 r of what the rotation mixes, |u c| + |v s|
+        // (the factor, the weight, the product), and r of itself through the last sum.  (|u c| + |v s|)^2 <= (u^2 + v^2) (c^2 + s^2) = x^2 + y^2, so that
+        // this is 9 r |x| + 3 r (|x| + |y|), no more than 7.2e-7 of |x| + |y|; the test below rounds once more, 0.6e-7.  Where 1.25e-6 of |x| + |y| less
+        // and as much more are not the same byte, or the maximum lies within 2^-18 of the next power's, the row is made over.
         care |= abs((int)(__float_as_uint(top) & 0x7fffffu) - 0x600000) < 32;
         const float slack = 1.25e-6f * back;
 #pragma unroll

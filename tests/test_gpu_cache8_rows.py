@@ -90,6 +90,45 @@ def test_rotated_rows_beyond_the_largest_number(way, d):
     equal(got, want, "keys")
 
 
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("norm", [True, False])
+def test_keys_next_to_borders(way, d, norm):
+    """Every number of a key within some tens of 2^-23 of itself of the middle between two 8-bit numbers, on either side, by the choice of the norm's weights
+    or of the rotation's table.  What separates the two sides is what 32 bits lose in a dozen roundings."""
+    n, n_q, n_kv, half = 48, 1, 1, d // 2
+    gen = torch.Generator().manual_seed(11)
+    keys = (torch.randn((n, 1, d), generator=gen, dtype=torch.float64)).to(torch.bfloat16)
+    keys = torch.where(keys == 0, torch.ones_like(keys), keys)
+    middle = (2 * torch.randint(8, 16, (n, d), generator=gen).double() + 1) / 16  # between m/8 and (m + 1)/8
+    middle = middle * 2.0 ** torch.randint(-5, 8, (n, d), generator=gen).double()
+    middle[:, 0] = 400.0  # every row's power is that of a maximum of 448 at most and more than 224
+    off = torch.randint(-40, 41, (n, d), generator=gen).double() * 2.0**-23
+    target = middle * (1 + off)
+    positions = list(range(n))
+    if norm:
+        # one row's weights are another's noise: each row is a call of its own
+        weight, cos, sin, eps = None, None, None, 1e-6
+        got, want = [], []
+        for i in range(0, n, 8):
+            x = keys[i, 0].double()
+            unit = x / torch.sqrt((x * x).mean() + eps)
+            weight = (target[i] / unit).float()
+            qkv = torch.cat([keys[i], keys[i], keys[i]]).to(torch.bfloat16).view(1, -1)
+            got.append(written(way, qkv, n_q, n_kv, d, eps, weight, None, None, [0])[0])
+            want.append(formula(keys[i:i + 1], weight, eps, None, None, [0]))
+        got, want = torch.cat(got), torch.cat(want)
+    else:
+        # c and s so that the first number of a pair comes out next to its middle: u c - v s = target
+        u, v = keys[:, 0, :half].double(), keys[:, 0, half:].double()
+        sin = (0.5 * torch.randn((n, half), generator=gen, dtype=torch.float64)).float()
+        cos = ((target[:, :half] + v * sin.double()) / u).float()
+        qkv = torch.cat([keys, keys, keys], 1).view(n, -1)
+        got, _ = written(way, qkv, n_q, n_kv, d, 1e-6, None, cos.contiguous(), sin.contiguous(), positions)
+        want = formula(keys, None, 0.0, cos, sin, positions)
+    equal(got, want, "keys")
+
+
 @pytest.mark.parametrize("n_q,n_kv,d", [(4, 2, 128), (6, 2, 64)])
 def test_a_position_outside_the_rotation_s_table(n_q, n_kv, d):
     """The decode kernel leaves such a token's key where it was, writes its value and reports it, as the write by itself does; the others are what they are."""
