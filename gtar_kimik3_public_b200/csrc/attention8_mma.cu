@@ -4,8 +4,9 @@
 // A row is a (token, query head of the kv head); up to 8 NT rows of a (sequence, kv head) are taken together, so that every key and value is
 // read once for all of them.  Both products are turned over, so that the rows are the eight columns of m16n8k16:
 //     S^T (16 keys x rows) = K8 Q^T          O^T (d x rows) += V8^T P^T
-// with e4m3 numbers as halves (exact), the queries as halves under a power of two of their row's own (exact but for numbers of 2^-28 of the row's
-// largest and less) and probabilities rounded to halves; sums are 32-bit.  A key's power of two multiplies its score, a value's goes into its
+// with e4m3 numbers as halves (exact), the queries as halves under a power of two of their row's own (bfloat16 ones exact but for numbers of 2^-28 of the
+// row's largest and less; those that the decode kernel has normed and rotated itself, in 32 bits, rounded by up to 2^-11 of each number, an eighth of what
+// bfloat16 would cost them) and probabilities rounded to halves; sums are 32-bit.  A key's power of two multiplies its score, a value's goes into its
 // probability.  So there are two running references a row:
 //     l  = sum_j 2^(s_j - A)               A near the largest s_j           (s in powers of two)
 //     o8 = sum_j 2^(s_j + ev_j - B) v8_j   B near the largest s_j + ev_j    out = o8 2^(B - A) / l
@@ -233,8 +234,6 @@ __device__ __forceinline__ void store4(__nv_bfloat16* to, const float4& v, float
     *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(two);
 }
 
-// A block's share of one (unit, kv head): the tiles tile_begin .. tile_end - 1.  `part` < 0: the whole of it or a cluster's split; else where its
-// sums go.
 // RMSNorm and rotation of a query whose columns 64 c + 16 t .. + 15 lane t of a quad holds.
 template <int D>
 __device__ __forceinline__ void norm_rotate_queries(const Fused8& f, float (&x)[D / 64][16], int pos, int t) {
@@ -321,6 +320,8 @@ __device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, cons
     __syncwarp();
 }
 
+// A block's share of one (unit, kv head): the tiles tile_begin .. tile_end - 1.  `part` < 0: the whole of it or a cluster's split; else where its
+// sums go.
 template <int D, int NT, bool FUSED>
 __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const Fused8& f, Smem8<D, NT>& sm, const Unit& u, int hk, int tile_begin, int tile_end, int split,
                                       int part) {

@@ -2549,7 +2549,8 @@ def qk_norm_rope_write8(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q
                         kv: PagedKV8, max_position: int, q_out: torch.Tensor | None = None, write_kv: bool = True) -> torch.Tensor:
     """``qk_norm_rope_write`` into 8-bit pages: per-head RMSNorm of q and k, rotation by position, and the write of k and v as e4m3 numbers
     with a power of two a (position, kv head) (see ``PagedKV8``).  Queries are 32-bit up to their one rounding; keys and values are kept as the
-    formula in 64 bits rounded once.  Returns the queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
+    formula in 64 bits rounded once.  (A row of queries whose squares leave 32 bits comes out as zeros, as from ``qk_norm_rope_write``.)  No two tokens of a
+    call may have the same place.  Returns the queries ``[n_tokens, n_q, head_dim]`` in the type of ``qkv`` (float32 or bfloat16)."""
     _check(qkv, "qkv", dims=2)
     n, width = qkv.shape
     if not (_fine8(kv, qkv, tok_pos, tok_seq, (n,)) and _fine8(kv, qkv, slots, slots, slots.shape) and slots.dim() == 1):
@@ -2681,8 +2682,8 @@ def attention_decode8_fused(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: in
                             max_position: int, max_kv_len: int, scale: float, window: int = 0, write_kv: bool = True,
                             cut: tuple[int, int] | None = None) -> torch.Tensor:
     """``qk_norm_rope_write8`` and ``attention_decode8`` of one new token per sequence in one kernel, from the packed projection
-    ``qkv [n_seqs, (n_q + 2 n_kv) * head_dim]`` (bfloat16, heads of 64 or 128, pages of 64).  The cache gets the same bytes; the queries are not
-    rounded to bfloat16 on the way.  No two sequences of the call may write into one page (with ``write_kv``, a slot stands in it once).  Returns ``[n_seqs, n_q, head_dim]``."""
+    ``qkv [n_seqs, (n_q + 2 n_kv) * head_dim]`` (bfloat16, heads of 64 or 128, pages of 64).  The cache gets the same bytes; the queries are normed and
+    rotated in 32 bits and rounded to halves under a power of two of their row (2^-11 of each number) in place of bfloat16 (2^-8).  No two sequences of the call may write into one page (with ``write_kv``, a slot stands in it once).  Returns ``[n_seqs, n_q, head_dim]``."""
     _check(qkv, "qkv", torch.bfloat16, 2)
     n = qkv.shape[0]
     if not _fine8(kv, qkv, kv_len, slots, (n,)):

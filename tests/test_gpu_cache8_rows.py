@@ -6,7 +6,7 @@ import torch
 
 from tests.plain import cache8 as plain8
 from tests.plain import model as plain
-from tests.test_gpu_cache8 import DEV, F, empty_pages, held, ints, rand
+from tests.test_gpu_cache8 import DEV, F, SINGLE, check_attention, empty_pages, fill, held, ints, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +150,27 @@ def test_a_position_outside_the_rotation_s_table(n_q, n_kv, d):
         assert torch.isnan(k[64]).all()  # the poison
     for name in ("k", "v", "k_exp", "v_exp"):
         assert torch.equal(getattr(pages[0], name).view(torch.uint8), getattr(pages[1], name).view(torch.uint8)), name
+
+
+@pytest.mark.parametrize("n_q,n_kv,d", [(8, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("cut", [(1, 0), (4, 0), (0, 40)])
+def test_queries_of_the_decode_kernel(n_q, n_kv, d, cut):
+    """Scores of some tens from queries that the kernel norms and rotates: they are rounded to halves, 2^-11 of each number, so a score may be off by 2^-11
+    of the sum of its products' sizes, and a probability by twice that of itself (once in the sum below it); 32-bit arithmetic in front of it loses 2^-20."""
+    lens, eps = [300, 64, 777], 1e-6
+    kv, slots, table = empty_pages(3, max(lens), n_kv, d)
+    for i, m in enumerate(lens):
+        fill(kv, table, int(slots[i]), rand(m - 1, n_kv, d, seed=30 + i, scale=3.0), rand(m - 1, n_kv, d, seed=60 + i))
+    qkv = rand(3, (n_q + 2 * n_kv) * d, seed=7).to(torch.bfloat16)
+    w = (3 + 0.3 * rand(d, seed=20)).float()
+    cos, sin = tables(max(lens), d)
+    got = F().attention_decode8_fused(qkv.to(DEV), n_q, n_kv, d, w.to(DEV), w.to(DEV), eps, cos.to(DEV), sin.to(DEV), kv, ints(*lens), slots, max(lens) - 1,
+                                      max(lens), d**-0.5, cut=cut)
+    F().check_kernel_errors(DEV)
+    x = formula(qkv.view(3, -1, d)[:, :n_q], w, eps, cos, sin, [m - 1 for m in lens])
+    for i, m in enumerate(lens):
+        k, v = held(kv, table, int(slots[i]), m)
+        sizes = torch.einsum("hd,jhd->hj", x[i].abs(), k.abs().repeat_interleave(n_q // n_kv, 1)) * d**-0.5
+        off = (2.0**-11 + 2.0**-20) * sizes.max().item()
+        assert off < 0.2
+        check_attention(got[i:i + 1], x[i:i + 1], k, v, m - 1, 0, False, SINGLE[torch.bfloat16] + torch.expm1(torch.tensor(2 * off)).item(), f"sequence of {m}")
