@@ -314,6 +314,11 @@ class Cache:
                 total += len(group.items) * r.n_kv_heads * (r.head_dim + (r.value_dim or r.head_dim)) * self.k_element_size()
         return total
 
+    @property
+    def keeps_8_bits(self) -> bool:
+        """Whether some layer's keys and values are kept in 8 bits."""
+        return any(getattr(g.request, "dtype", None) is not None for g in self.kv_groups)
+
     def scratch_bytes_per_token(self) -> int:
         """What a step may need for a moment besides the cache, for each token that it holds: prompts attend over one layer's 8-bit pages at a time
         made bfloat16."""

@@ -16,6 +16,10 @@ cache made for long ones is not cut into as many pieces as the longest context w
 launch shape is a matter of speed only (into how many blocks a sequence's pages are cut), it is chosen
 for the middle of the lengths that the bound covers.
 
+Steps of several tokens a sequence over keys and values in 8 bits carry such a bound too (256, 384, 512, ...): pages are made clean, and
+kernels chosen, by it (``prompt8_length``, which gives for the bound what it gives for the lengths themselves).  Over other caches nothing in such a
+step goes by the longest length, and the cache's own stands in.
+
 A step is executed exactly once, also the step at which its shape is captured: that step runs launch
 by launch (which does whatever one-time set-up the kernels need) and gives the result, the capture
 after it executes nothing, and replays serve the later steps.  A part that advances a state in place
@@ -35,7 +39,7 @@ import numpy as np
 import torch
 
 from ..ops import library
-from ..ops.functional import copy_to_device, set_pdl
+from ..ops.functional import PROMPT8_LEAST_BOUND, copy_to_device, length_class, set_pdl
 from .step import PackedStep, context_from_views
 
 
@@ -122,20 +126,23 @@ class StepGraphs:
         longest = self.cache.max_seq_len
         if not packed.all_single:
             return longest, 0
-        below, bound = 0, self.MIN_LENGTH_BOUND
-        while bound < packed.max_kv_len:
-            # 1, 1.5, 2, 3, 4, 6, ... times the least bound
-            below, bound = bound, (bound * 3 // 2 if bound & (bound - 1) == 0 else bound * 4 // 3)
+        below, bound = length_class(packed.max_kv_len, self.MIN_LENGTH_BOUND)
         bound = min(bound, longest)
         return bound, max(1, (below + bound + 1) // 2)
 
     def length_bound(self, packed: PackedStep) -> int:
         return self.length_bounds(packed)[0]
 
+    def launch_bounds(self, packed: PackedStep) -> tuple[int, int]:
+        """``length_bounds`` of a captured step; several tokens a sequence over 8-bit keys and values have a bound of their own."""
+        if packed.all_single or not self.cache.keeps_8_bits:
+            return self.length_bounds(packed)
+        return min(length_class(packed.max_kv_len, PROMPT8_LEAST_BOUND)[1], self.cache.max_seq_len), 0
+
     def key_of(self, packed: PackedStep) -> tuple:
         if packed.all_single:
             return (packed.n_tokens, packed.n_seqs, packed.n_want, 1, self.length_bound(packed))
-        return (packed.n_tokens, packed.n_seqs, packed.n_want, packed.max_q_len, 0)
+        return (packed.n_tokens, packed.n_seqs, packed.n_want, packed.max_q_len, self.launch_bounds(packed)[0] if self.cache.keeps_8_bits else 0)
 
     def wants_graph(self, packed: PackedStep, key: tuple | None = None) -> bool:
         """Decode shapes always; other shapes from their second appearance on."""
@@ -169,7 +176,7 @@ class StepGraphs:
         logits of the run (the capture itself executes nothing, so the step has run once)."""
         self.model.prepare(self.cache.max_seq_len - 1)
         # launch shapes inside a graph must not depend on the lengths of the day: a bound stands in
-        bound, typical = self.length_bounds(packed)
+        bound, typical = self.launch_bounds(packed)
         ctx = context_from_views(packed, self.views(packed), self.model.dtype, max_kv_len=bound, typical_kv_len=typical)
         step = self.model.step if self.use_pdl else library.in_order(self.model.step)
         result = step(ctx, self.cache)  # one-time set-up happens here, outside the capture

@@ -2721,6 +2721,26 @@ def attention_decode8(q: torch.Tensor, kv: PagedKV8, kv_len: torch.Tensor, slots
     return out
 
 
+PROMPT8_LEAST_BOUND = 256
+
+
+@functools.lru_cache(maxsize=4096)
+def length_class(length: int, least: int) -> tuple[int, int]:
+    """The lengths ``below < length <= bound`` that count as one: 1, 1.5, 2, 3, 4, 6, ... times ``least``."""
+    below, bound = 0, least
+    while bound < length:
+        below, bound = bound, (bound * 3 // 2 if bound & (bound - 1) == 0 else bound * 4 // 3)
+    return below, bound
+
+
+def prompt8_length(max_kv_len: int, max_q_len: int, window: int = 0) -> int:
+    """The length that several tokens a sequence have their kernel and its cut chosen by: the middle of the class of the longest.  A step captured for a bound
+    that is in the class takes the kernel, and gives the bits, that it takes by its true lengths."""
+    below, bound = length_class(int(max_kv_len), PROMPT8_LEAST_BOUND)
+    middle = max((below + bound + 1) // 2, max_q_len)
+    return min(middle, window + max_q_len) if window else middle
+
+
 @functools.lru_cache(maxsize=4096)
 def rows8_wins(n_tokens: int, n_seqs: int, max_q_len: int, max_kv_len: int, n_kv: int, group: int, d: int, sm_count: int) -> bool:
     """Whether several tokens a sequence go through the kernel for few rows (16 at a time, every tile reading its keys by itself) and not through pages
@@ -2775,7 +2795,7 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
                        scale: float, window: int = 0, sink: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the packed new tokens ``q [n_tokens, n_q, d]`` (bfloat16 or float32) over 8-bit pages.  Sequence ``i`` owns the tokens
     ``cu_q[i] .. cu_q[i+1]-1``, its last positions: ``kv_len[i]`` counts its cached tokens including them.  ``max_q_len`` and ``max_kv_len`` are the
-    largest of both, or bounds.  Rows of ``out`` behind the last sequence are left as they were.  A sequence with more tokens than positions or than
+    largest of both, or bounds (by ``max_kv_len`` the kernel is chosen: ``prompt8_length``).  Rows of ``out`` behind the last sequence are left as they were.  A sequence with more tokens than positions or than
     ``max_q_len`` is reported; tokens in front of its first position get zeros."""
     out = _check_queries8(q, kv, out)
     n_seqs = kv_len.shape[0]
@@ -2785,8 +2805,9 @@ def attention_prefill8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor, kv_len
     _, n_kv, page, _ = kv._sizes
     group = n_q // n_kv
     if q.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and group <= ROWS8_MAX_GROUP and n_seqs and n_tokens:
-        if rows8_wins(n_tokens, n_seqs, max_q_len, min(max_kv_len, window + max_q_len) if window else max_kv_len, n_kv, group, d, _sm_count_of(kv._index)):
-            return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), max_kv_len, scale, window, sink, None, out)
+        length = prompt8_length(max_kv_len, max_q_len, window)
+        if rows8_wins(n_tokens, n_seqs, max_q_len, length, n_kv, group, d, _sm_count_of(kv._index)):
+            return _rows8(q, kv, cu_q, kv_len, slots, max(1, max_q_len), length, scale, window, sink, None, out)
         return _prefill_clean8(q, kv, cu_q, kv_len, slots, max_q_len, max_kv_len, scale, window, sink, out)
     call("gk_attend8", kv._at, ptr(q), dtype_code(q.dtype), ptr(out), ptr(cu_q), ptr(kv_len), ptr(slots), q.shape[0], n_seqs, q.shape[1], float(scale),
          int(window), int(sink), stream_ptr())
