@@ -389,9 +389,9 @@ __global__ void __launch_bounds__(256) read8_kernel(const GkPages8 p, const int*
         }
     }
     long long back = last;  // how many of the sequence's last positions are wanted (0: all)
-    if (CLEAN && clean.window > 0) {  // those that its first token sees, and on; starts that are put in order make no sequence longer
+    if (CLEAN && clean.window > 0) {  // those that its first token sees, itself among them, and on; starts that are put in order make no sequence longer
         const int from = max(clean.cu_q_in[seq], 0), to = min(clean.cu_q_in[seq + 1], clean.n_tokens);
-        back = (long long)clean.window + max(0, to - from);
+        back = max((long long)clean.window + max(0, to - from) - 1, 1LL);
     }
     const bool seen = (long long)index * p.page_size < len && (back <= 0 || (index + 1) * (long long)p.page_size > (long long)len - back);
     const int page = seen ? page_of(p, slots[seq], index) : -1;

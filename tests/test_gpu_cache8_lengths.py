@@ -142,3 +142,19 @@ def test_a_window_over_more_tokens_than_max_q_len(way, d):
         F().check_kernel_errors(DEV)
     k, v = held(kv, table, int(slots[0]), n)
     check_attention(out[-8:], q[-8:], k, v, n - 8, window, False, SEVERAL[way], "the last tokens")
+
+
+@pytest.mark.parametrize("way", ["few", "clean", "any"], indirect=True)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("past,pages", [(73, 1), (74, 1), (137, 2)])
+def test_pages_that_the_window_has_left_are_not_looked_at(way, d, past, pages):
+    """Up to the page whose last position is the one right in front of the window: no page number stands for them any more."""
+    window, new, n_q, n_kv = 10, 5, 4, 2
+    kv, slots, table = sequences([past + new, 30], n_kv, d)
+    kv.block_table[slots[0].long(), :pages] = -1
+    q = rand(new + 2, n_q, d, seed=5).to(way)
+    got = F().attention_prefill8(q.to(DEV), kv, ints(0, new, new + 2), ints(past + new, 30), slots, new, past + new, d**-0.5, window)
+    F().check_kernel_errors(DEV)
+    for i, (at, m, n) in enumerate([(0, new, past + new), (new, 2, 30)]):
+        k, v = held(kv, table, int(slots[i]), n)
+        check_attention(got[at:at + m], q[at:at + m], k, v, n - m, window, False, SEVERAL[way], f"sequence {i}")
