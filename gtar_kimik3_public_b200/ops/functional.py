@@ -2671,10 +2671,12 @@ def _rows8(q: torch.Tensor, kv: PagedKV8, cu_q: torch.Tensor | None, kv_len: tor
     return out
 
 
-def decode8_fused_ok(qkv: torch.Tensor, kv: PagedKV8, n_q: int) -> bool:
-    """Whether the decode kernel that also norms, rotates and writes the new token takes the layer."""
+def decode8_fused_ok(qkv: torch.Tensor, kv: PagedKV8, n_q: int, *vectors: torch.Tensor | None) -> bool:
+    """Whether the decode kernel that also norms, rotates and writes the new token takes the layer; ``vectors``: its norm weights and tables, which that
+    kernel reads sixteen bytes at a time."""
     _, n_kv, page, d = kv._sizes
-    return qkv.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and n_q // n_kv <= ROWS8_MAX_GROUP
+    return (qkv.dtype is torch.bfloat16 and d in ROWS8_HEAD_DIMS and page == 64 and n_q // n_kv <= ROWS8_MAX_GROUP
+            and not any([t is not None and t.data_ptr() & 15 for t in vectors]))
 
 
 def attention_decode8_fused(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,

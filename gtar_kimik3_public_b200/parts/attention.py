@@ -130,7 +130,7 @@ class GQAAttention(Mixer):
     def _attend(self, qkv: torch.Tensor, ctx: StepContext, cache: F.PagedKV, cos, sin, write_kv: bool) -> torch.Tensor:
         """Attention output ``[n_tokens, n_q, head_dim]`` from the packed projection of the step's tokens."""
         if isinstance(cache, F.PagedKV8):
-            if ctx.all_single and F.decode8_fused_ok(qkv, cache, self.n_q):
+            if ctx.all_single and F.decode8_fused_ok(qkv, cache, self.n_q, self.q_norm, self.k_norm, cos, sin):
                 return F.attention_decode8_fused(
                     qkv, self.n_q, self.n_kv, self.head_dim, self.q_norm, self.k_norm, self.qk_norm_eps or 1.0, cos, sin, cache, ctx.kv_len, ctx.slots,
                     ctx.max_position, ctx.typical_kv_len or ctx.max_kv_len, self.scale, self.window or 0, write_kv)

@@ -174,3 +174,33 @@ def test_queries_of_the_decode_kernel(n_q, n_kv, d, cut):
         off = (2.0**-11 + 2.0**-20) * sizes.max().item()
         assert off < 0.2
         check_attention(got[i:i + 1], x[i:i + 1], k, v, m - 1, 0, False, SINGLE[torch.bfloat16] + torch.expm1(torch.tensor(2 * off)).item(), f"sequence of {m}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_layer_whose_norm_weights_begin_anywhere(d):
+    """Weights that begin between sixteen bytes: the decode kernel that norms refuses them, and a layer takes the write and the attention instead."""
+    from types import SimpleNamespace
+
+    from gtar_kimik3_public_b200.parts import build_part
+
+    n_q, n_kv, lens = 4, 2, [70, 5]
+    mixer = build_part("mixer", "gqa_attention", hidden_size=64, n_q_heads=n_q, n_kv_heads=n_kv, head_dim=d, qk_norm_eps=1e-6, position=None)
+    both = (1 + 0.1 * rand(2 * d + 3, seed=4)).to(torch.bfloat16).to(DEV)
+    mixer.q_norm, mixer.k_norm = both[1:d + 1], both[d + 3:2 * d + 3]
+    qkv = rand(2, (n_q + 2 * n_kv) * d, seed=7).to(torch.bfloat16).to(DEV)
+    got = []
+    for layer in (True, False):
+        kv, slots, table = empty_pages(2, max(lens), n_kv, d)
+        for i, m in enumerate(lens):
+            fill(kv, table, int(slots[i]), rand(m - 1, n_kv, d, seed=30 + i), rand(m - 1, n_kv, d, seed=60 + i))
+        at, seq, kv_len = ints(*[m - 1 for m in lens]), ints(0, 1), ints(*lens)
+        if layer:
+            with pytest.raises(F().KernelError, match="16-byte"):
+                F().attention_decode8_fused(qkv, n_q, n_kv, d, mixer.q_norm, mixer.k_norm, 1e-6, None, None, kv, kv_len, slots, 69, 70, d**-0.5)
+            ctx = SimpleNamespace(all_single=True, tok_pos=at, tok_seq=seq, kv_len=kv_len, slots=slots, max_position=69, max_kv_len=70, typical_kv_len=0)
+            got.append(mixer._attend(qkv, ctx, kv, None, None, True))
+        else:
+            q = F().qk_norm_rope_write8(qkv, n_q, n_kv, d, mixer.q_norm, mixer.k_norm, 1e-6, None, None, at, seq, slots, kv, 69)
+            got.append(F().attention_decode8(q, kv, kv_len, slots, 70, d**-0.5))
+    F().check_kernel_errors(DEV)
+    assert torch.equal(got[0], got[1])
