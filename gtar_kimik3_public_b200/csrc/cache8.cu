@@ -113,7 +113,7 @@ __device__ __forceinline__ void finish_row(const GkPages8& p, const Write8& a, f
                                            const float (&w1)[HD / 16], const float (&c)[HD / 16], const float (&sn)[HD / 16], bool turns, bool is_v,
                                            __nv_bfloat16* q_out, const __nv_bfloat16* in, int pos, long long place, int sub, unsigned mask) {
     constexpr int E = HD / 16, HALF = HD / 2;
-    const bool lost = !is_v && norm_rotate_32<HD>(a, x, y, w0, w1, c, sn, turns, mask);
+    if (!is_v) norm_rotate_32<HD>(a, x, y, w0, w1, c, sn, turns, mask);
     if (q_out) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -129,7 +129,7 @@ __device__ __forceinline__ void finish_row(const GkPages8& p, const Write8& a, f
         return;
     }
     uint32_t four[2][E / 4];
-    const int b = make_bytes<HD, TW>(a, x, y, turns, is_v, lost, in, pos, sub, mask, four);
+    const int b = make_bytes<HD, TW>(a, x, y, turns, is_v, in, pos, sub, mask, four);
     uint8_t* to = (is_v ? p.v : p.k) + place * HD + sub * E;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {

@@ -137,14 +137,15 @@ __device__ __forceinline__ float to_be_rounded(float high, float low) {
     return __uint_as_float((__float_as_uint(h) - ((l < 0.f) != (h < 0.f) ? 1u : 0u)) | 1u);
 }
 
-constexpr float LARGEST = 3.402823466e38f, LARGE_SQUARES = 0x1p120f;
-constexpr float SMALL_MEAN = 0x1p-60f;  // below it the mean of squares and eps lose bits of squares that end at 2^-149
+constexpr float LARGEST = 3.402823466e38f;
 
 // A key, or a row of values as it is, by LANES lanes that have HD / 2 / LANES neighbouring numbers of each half: the numbers to be rounded; the byte of the
-// row's power comes back.
+// row's power comes back.  By a whole warp rows of any size; by fewer lanes (where the registers that this takes cost the write more) only rows whose
+// squares and rotation stay within 32 bits: `far_bytes`.
 template <int HD, int LANES, typename TW>
 __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, float (&x)[2][HD / 2 / LANES]) {
     constexpr int E = HD / 2 / LANES, HALF = HD / 2;
+    constexpr bool ANY = LANES == 32;
     float low[2][E];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -173,23 +174,23 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
             };
             Two8 ss = squares();
             float eps = a.eps;
-            if (!(ss.h < LARGE_SQUARES) || (ss.h < SMALL_MEAN && eps < SMALL_MEAN)) {  // (the same for the lanes of the row)
+            if (ANY && (!(ss.h < 0x1p120f) || (ss.h < 0x1p-60f && eps < 0x1p-60f))) {  // (the same for the lanes of the row)
                 // Squares that leave 32 bits: the row times a power of two, and eps times its square, come to the same.  The row's largest finite number
                 // becomes one of 1 to 2, or less where eps would leave 32 bits; what of eps is lost is nothing beside the squares then.
-                float top = 0.f;
+                float most = 0.f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < E; ++i) top = fmaxf(top, finite_abs(x[h][i]));
+                    for (int i = 0; i < E; ++i) most = fmaxf(most, finite_abs(x[h][i]));
 #pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
-                const int up = min(127 - (int)(__float_as_uint(top) >> 23), eps > 0.f ? 50 - ((int)(__float_as_uint(eps) >> 23) - 127) / 2 : 120);
-                const float half = __uint_as_float((uint32_t)(127 + up / 2) << 23), rest = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);  // 2^up in two factors
-                eps = ((eps * half) * half) * rest * rest;
+                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
+                const int up = min(127 - (int)(__float_as_uint(most) >> 23), eps > 0.f ? 50 - ((int)(__float_as_uint(eps) >> 23) - 127) / 2 : 120);
+                const float part = __uint_as_float((uint32_t)(127 + up / 2) << 23), rest = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);  // 2^up in two factors
+                eps = eps * part * part * rest * rest;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < E; ++i) x[h][i] = (x[h][i] * half) * rest;
+                    for (int i = 0; i < E; ++i) x[h][i] = (x[h][i] * part) * rest;
                 ss = squares();
             }
             const Two8 m = sum_of(ss.h * (1.f / HD), eps);  // (HD is a power of two)
@@ -225,7 +226,7 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
                     const Two8 p = product_of(h ? v : u, c[i]), q = product_of(h ? u : v, s), t = sum_of(p.h, q.h);
                     x[h][i] = t.h;
                     low[h][i] = __fadd_rn(__fadd_rn(t.l, __fadd_rn(p.l, q.l)), __fmaf_rn(h ? vl : ul, c[i], __fmul_rn(h ? ul : vl, s)));
-                    if (fabsf(t.h) == INFINITY && fabsf(u) < INFINITY && fabsf(v) < INFINITY) {  // of finite numbers: the largest that there is
+                    if (ANY && fabsf(t.h) == INFINITY && fabsf(u) < INFINITY && fabsf(v) < INFINITY) {  // of finite numbers: the largest that there is
                         x[h][i] = copysignf(LARGEST, t.h);
                         low[h][i] = 0.f;
                     }
@@ -245,10 +246,53 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
     for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
     return exponent_byte(top);
 }
-// The same by eight lanes, as bytes.
+// A key by eight lanes, as bytes: of any size, in 64 bits, a number after the other.
 template <int HD, typename TW>
-__device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, uint32_t* four) {
+__device__ __noinline__ int far_bytes(const Norm8& a, const __nv_bfloat16* row, int pos, int sub, unsigned mask, uint32_t* four) {
+    constexpr int E = HD / 16, HALF = HD / 2;
+    const bool turns = a.cos_table && (unsigned)pos < (unsigned)a.table_positions;
+    double inv = 1.0;
+    if (a.use_norm) {
+        double ss = 0.0;
+#pragma unroll 1
+        for (int i = 0; i < 2 * E; ++i) {
+            const double x = __bfloat162float(row[(i < E ? i : HALF - E + i) + sub * E]);
+            ss += x * x;
+        }
+        for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
+        inv = 1.0 / sqrt(ss / HD + (double)a.eps);
+    }
+    float top = 0.f, back = 0.f;
+    int b = 0;
+#pragma unroll 1
+    for (int i = 0; i < 4 * E; ++i) {  // twice through the lane's numbers: the maximum, the bytes
+        const int h = i / E % 2, c = sub * E + i % E;
+        if (i == 2 * E) {
+            for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+            b = exponent_byte(top);
+            back = power_back(b);
+        }
+        double u = __bfloat162float(row[c]), v = __bfloat162float(row[HALF + c]);
+        if (a.use_norm) {
+            u = (u * inv) * (double)to_float(((const TW*)a.wk)[c]);
+            v = (v * inv) * (double)to_float(((const TW*)a.wk)[HALF + c]);
+        }
+        double x = h ? v : u;
+        if (turns) {
+            const double co = a.cos_table[(size_t)pos * HALF + c], si = a.sin_table[(size_t)pos * HALF + c];
+            x = h ? v * co + u * si : u * co - v * si;
+        }
+        const float f = to_be_rounded(x);
+        if (i < 2 * E) top = fmaxf(top, finite_abs(f));
+        else reinterpret_cast<unsigned char*>(four)[i - 2 * E] = (unsigned char)pack2(f * back, 0.f);
+    }
+    return b;
+}
+// The careful row by eight lanes, as bytes.
+template <int HD, typename TW>
+__device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, bool far, int pos, int sub, unsigned mask, uint32_t* four) {
     constexpr int E = HD / 16;
+    if (far) return far_bytes<HD, TW>(a, row, pos, sub, mask, four);
     float x[2][E];
     const int b = careful_row<HD, 8, TW>(a, row, is_v, pos, sub, mask, x);
     const float back = power_back(b);
@@ -260,19 +304,16 @@ __device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* r
     return b;
 }
 
-// RMSNorm and rotation of a row in 32 bits.  Returns whether its mean of squares has lost bits at the range's lower end (one that leaves the upper end makes
-// the row zeros, which `make_bytes` sees).
+// RMSNorm and rotation of a row in 32 bits.
 template <int HD>
-__device__ __forceinline__ bool norm_rotate_32(const Norm8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16], const float (&w1)[HD / 16],
+__device__ __forceinline__ void norm_rotate_32(const Norm8& a, float (&x)[HD / 16], float (&y)[HD / 16], const float (&w0)[HD / 16], const float (&w1)[HD / 16],
                                                const float (&c)[HD / 16], const float (&sn)[HD / 16], bool turns, unsigned mask) {
     constexpr int E = HD / 16;
-    bool lost = false;
     if (a.use_norm) {
         float ss = sum_of_squares(x, y);
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float mean = fmaf(ss, 1.f / HD, a.eps), inv = rsqrtf(mean);
-        lost = mean < SMALL_MEAN;
+        const float inv = rsqrtf(fmaf(ss, 1.f / HD, a.eps));
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             x[i] = (x[i] * inv) * w0[i];
@@ -287,14 +328,12 @@ __device__ __forceinline__ bool norm_rotate_32(const Norm8& a, float (&x)[HD / 1
             y[i] = v * c[i] + u * sn[i];
         }
     }
-    return lost;
 }
 
-// A lane's bytes of a key (normed and rotated in 32 bits, `row` what it was made of, `lost` as above) or of a row of values; the byte of the row's power
-// comes back.
+// A lane's bytes of a key (normed and rotated in 32 bits, `row` what it was made of) or of a row of values; the byte of the row's power comes back.
 template <int HD, typename TW>
-__device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 16], const float (&y)[HD / 16], bool turns, bool is_v, bool lost,
-                                          const __nv_bfloat16* row, int pos, int sub, unsigned mask, uint32_t (&four)[2][HD / 64]) {
+__device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 16], const float (&y)[HD / 16], bool turns, bool is_v, const __nv_bfloat16* row,
+                                          int pos, int sub, unsigned mask, uint32_t (&four)[2][HD / 64]) {
     constexpr int E = HD / 16;
     float top = 0.f;
 #pragma unroll
@@ -303,8 +342,10 @@ __device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 
     for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
     const int b = exponent_byte(top);
     const float back = power_back(b);
-    // (a row that holds an infinity or NaN and is normed: its maximum is 0 or not to be trusted)
-    bool care = top == INFINITY || lost || (!is_v && a.use_norm && top == 0.f);
+    // a row whose maximum is 0 or not to be trusted: it holds an infinity or NaN and is normed, its squares leave 32 bits (zeros come of it; or, with next
+    // to no eps, lost bits), or its rotation does
+    const bool far = !is_v && (top >= 0x1p127f || (a.use_norm && (top == 0.f || a.eps < 0x1p-60f)));  // (the same for the lanes of the row)
+    bool care = far || top == INFINITY;
     if (is_v || !(a.use_norm || turns)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -341,7 +382,7 @@ __device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 
     }
     if (__any_sync(mask, care)) {
         uint32_t anew[2 * (E / 4)];
-        const int power = careful_bytes<HD, TW>(a, row, is_v, pos, sub, mask, anew);
+        const int power = careful_bytes<HD, TW>(a, row, is_v, far, pos, sub, mask, anew);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
