@@ -11,7 +11,9 @@
 //     l  = sum_j 2^(s_j - A)               A near the largest s_j           (s in powers of two)
 //     o8 = sum_j 2^(s_j + ev_j - B) v8_j   B near the largest s_j + ev_j    out = o8 2^(B - A) / l
 // A and B are moved only when a number would pass 2^14 or 2^15 (halves end at 65,504): after a sequence's first keys hardly ever, and then no lane
-// has to ask the others for a maximum.  B is set 7 below the largest, so that probabilities keep all their bits down to 2^-21 of it.
+// has to ask the others for a maximum.  B is set 7 below the largest, so that probabilities keep all their bits down to 2^-21 of it.  Where a tile's
+// values are more than 2^7 smaller than those that B goes by (a column in which the large ones have nothing would show what is lost), what the halves of
+// probabilities above 2^-32 leave over is added by itself.  (To look for such tiles costs 64 sequences of 1,024 to 8,192 tokens 0.4 of 101 us.)
 //
 // The contraction over d may take d in any order that both operands share, and the keys of a product any order that P and V share: lane (g, t) =
 // (lane / 4, lane % 4) reads sixteen bytes in one piece of the keys 4g .. 4g + 3, and of the values 8t .. 8t + 7 its own sixteen (or eight) columns,
@@ -133,6 +135,12 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t turned(uint32_t x) {  // an 8 x 8 matrix of halves, rows for columns
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -142,6 +150,15 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t low_bf16(uint32_t four) {  // (exact)
+    const float2 two = floats2((uint16_t)four);
+    return pack_bf16(two.x, two.y);
 }
 __device__ __forceinline__ uint32_t low_halves(uint32_t four) { return halves2((uint16_t)four); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t four) { return halves2((uint16_t)(four >> 16)); }
@@ -434,6 +451,7 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
 #pragma unroll
     for (int i = 0; i < 8; ++i) v_at[i] = At::value(8 * t + i, D / 8 * g);
     uint32_t place = ring;
+    float gap = -INFINITY;  // the largest B - A of this lane's rows
 #pragma unroll 1
     for (; at < tile_end; at += WARPS) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -524,35 +542,84 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
                     }
                 beyond |= ma > ref_a[n][i] + 14.f || mb > ref_b[n][i] + 15.f;
             }
-        if (__any_sync(0xffffffffu, beyond)) {
+        const float least = fminf(fminf(ev[0], ev[1]), fminf(ev[2], ev[3]));  // below the gap: values that are small beside those that B goes by
+        if (__any_sync(0xffffffffu, beyond || least < gap)) {
+            if (__any_sync(0xffffffffu, beyond)) {
+                gap = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float ma = -INFINITY, mb = -INFINITY;
+                    for (int i = 0; i < 2; ++i) {
+                        float ma = -INFINITY, mb = -INFINITY;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                ma = fmaxf(ma, s[h][n][i + 2 * j]);
+                                mb = fmaxf(mb, s[h][n][i + 2 * j] + ev[2 * h + j]);
+                            }
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) {
+                            ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, w));
+                            mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, w));
+                        }
+                        const float na = fmaxf(ref_a[n][i], ma), nb = fmaxf(ref_b[n][i], mb - 7.f);
+                        const float fa = exp2_fast(ref_a[n][i] - na), fb = exp2_fast(ref_b[n][i] - nb);
+                        l[n][i] *= fa;
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            o[n][m][i] *= fb;
+                            o[n][m][2 + i] *= fb;
+                        }
+                        ref_a[n][i] = na;
+                        ref_b[n][i] = nb;
+                        if (na > NONE) gap = fmaxf(gap, nb - na);
+                    }
+            }
+            if (__builtin_expect(__any_sync(0xffffffffu, least < gap), 0)) {
+                // What the halves of small probabilities leave over, as the sum of two bfloat16 numbers (which reach as far down as 32 bits do) times values
+                // in bfloat16 (exact).  In a loop, for its code stands in the way of all the other tiles'.
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t high[NT][2], low[NT][2];
+                    bool some = false;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            ma = fmaxf(ma, s[h][n][i + 2 * j]);
-                            mb = fmaxf(mb, s[h][n][i + 2 * j] + ev[2 * h + j]);
+                            float rest[2];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const float score = h ? s[1][n][2 * j + i] : s[0][n][2 * j + i], x = exp2_fast(score + ((h ? ev[2 + j] : ev[j]) - ref_b[n][i]));
+                                rest[i] = x < 0x1p-14f && score > ref_a[n][i] - 32.f ? x - __half2float(__float2half_rn(x)) : 0.f;
+                                some |= rest[i] != 0.f;
+                            }
+                            const uint32_t two = pack_bf16(rest[0], rest[1]);
+                            high[n][j] = turned(two);
+                            low[n][j] = turned(pack_bf16(rest[0] - __uint_as_float(two << 16), rest[1] - __uint_as_float(two & 0xffff0000u)));
+                        }
+                    if (!__any_sync(0xffffffffu, some)) continue;
+#pragma unroll
+                    for (int w = 0; w < D / 32; ++w) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int mine = 2 * h + (i & 1) * 4 + (i >> 1);
+                            v[i] = none >> (8 * t + mine) & 1 ? 0u : read_word(place + (h ? v_at[2 + (i & 1) * 4 + (i >> 1)] : v_at[(i & 1) * 4 + (i >> 1)]) + 4 * w);
                         }
 #pragma unroll
-                    for (int w = 4; w < 32; w <<= 1) {
-                        ma = fmaxf(ma, __shfl_xor_sync(0xffffffffu, ma, w));
-                        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, w));
-                    }
-                    const float na = fmaxf(ref_a[n][i], ma), nb = fmaxf(ref_b[n][i], mb - 7.f);
-                    const float fa = exp2_fast(ref_a[n][i] - na), fb = exp2_fast(ref_b[n][i] - nb);
-                    l[n][i] *= fa;
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t near = __byte_perm(v[0], v[1], e ? 0x7362 : 0x5140), far = __byte_perm(v[2], v[3], e ? 0x7362 : 0x5140);
+                            const uint32_t a0 = low_bf16(near), a1 = low_bf16(near >> 16), a2 = low_bf16(far), a3 = low_bf16(far >> 16);
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        o[n][m][i] *= fb;
-                        o[n][m][2 + i] *= fb;
+                            for (int n = 0; n < NT; ++n) {
+                                mma_bf16(o[n][2 * w + e], a0, a1, a2, a3, high[n][0], high[n][1]);
+                                mma_bf16(o[n][2 * w + e], a0, a1, a2, a3, low[n][0], low[n][1]);
+                            }
+                        }
                     }
-                    ref_a[n][i] = na;
-                    ref_b[n][i] = nb;
                 }
+            }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
