@@ -310,6 +310,8 @@ __device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, cons
     int b[2];
 #pragma unroll
     for (int v = 0; v < 2; ++v) b[v] = careful_row<D, 32, TW>(f, row + (size_t)v * p.n_kv * D, v == 1, pos, lane, 0xffffffffu, x[v]);
+    const bool far = b[0] >= FAR_ROW;
+    if (far) b[0] -= FAR_ROW;
     const int page = page_of(p, u.slot, pos / PAGE);
     const size_t place = ((size_t)max(page, 0) * p.n_kv + hk) * PAGE + pos % PAGE;
 #pragma unroll
@@ -320,7 +322,8 @@ __device__ __forceinline__ void new_rows(const GkPages8& p, const Rows8& a, cons
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int at = h * HALF + lane * E;
-            const uint32_t two = pack2(x[v][h][0] * back, x[v][h][E - 1] * back);
+            uint32_t two = pack2(x[v][h][0] * back, x[v][h][E - 1] * back);
+            if (v == 0 && far) two = far_pair(two);
             if constexpr (E == 2) {
                 *reinterpret_cast<uint16_t*>(&bytes[v][at]) = (uint16_t)two;
                 if (kept) *reinterpret_cast<uint16_t*>(to + at) = (uint16_t)two;

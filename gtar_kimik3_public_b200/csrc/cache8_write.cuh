@@ -138,14 +138,21 @@ __device__ __forceinline__ float to_be_rounded(float high, float low) {
 }
 
 constexpr float LARGEST = 3.402823466e38f;
+// The squares of a row whose largest number is below SMALL_ROW end at 2^-149 with bits that count, where eps does not outweigh them; below LARGE_ROW no sum of
+// squares leaves 32 bits.
+constexpr float SMALL_EPS = 0x1p-60f, SMALL_ROW = 0x1p-26f, LARGE_ROW = 0x1p60f;
 
 // A key, or a row of values as it is, by LANES lanes that have HD / 2 / LANES neighbouring numbers of each half: the numbers to be rounded; the byte of the
-// row's power comes back.  By a whole warp rows of any size; by fewer lanes (where the registers that this takes cost the write more) only rows whose
-// squares and rotation stay within 32 bits: `far_bytes`.
+// row's power comes back.  By a whole warp rows of any size (FAR_ROW is added where squares had left 32 bits); by fewer lanes (where the registers that this
+// takes cost the write more) only rows whose squares and rotation stay within 32 bits: the others are for `far_bytes`.
+constexpr int FAR_ROW = 256;
+// Two bytes of a far row: a zero has no sign, for the two ways of making it do not keep the same ones.
+__device__ __forceinline__ uint32_t far_pair(uint32_t two) { return two & ~(__vcmpeq4(two & 0x7f7fu, 0u) & 0x8080u); }
 template <int HD, int LANES, typename TW>
 __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* row, bool is_v, int pos, int sub, unsigned mask, float (&x)[2][HD / 2 / LANES]) {
     constexpr int E = HD / 2 / LANES, HALF = HD / 2;
     constexpr bool ANY = LANES == 32;
+    bool far = false;
     float low[2][E];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -174,9 +181,7 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
             };
             Two8 ss = squares();
             float eps = a.eps;
-            if (ANY && (!(ss.h < 0x1p120f) || (ss.h < 0x1p-60f && eps < 0x1p-60f))) {  // (the same for the lanes of the row)
-                // Squares that leave 32 bits: the row times a power of two, and eps times its square, come to the same.  The row's largest finite number
-                // becomes one of 1 to 2, or less where eps would leave 32 bits; what of eps is lost is nothing beside the squares then.
+            if (ANY && (!(ss.h < INFINITY) || eps < SMALL_EPS)) {  // (the same for the lanes of the row)
                 float most = 0.f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -184,14 +189,19 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
                     for (int i = 0; i < E; ++i) most = fmaxf(most, finite_abs(x[h][i]));
 #pragma unroll
                 for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
-                const int up = min(127 - (int)(__float_as_uint(most) >> 23), eps > 0.f ? 50 - ((int)(__float_as_uint(eps) >> 23) - 127) / 2 : 120);
-                const float part = __uint_as_float((uint32_t)(127 + up / 2) << 23), rest = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);  // 2^up in two factors
-                eps = eps * part * part * rest * rest;
+                far = !(ss.h < INFINITY) || (most > 0.f && most < SMALL_ROW);
+                if (far) {
+                    // Squares that leave 32 bits: the row times a power of two, and eps times its square, come to the same.  The row's largest finite number
+                    // becomes one of 1 to 2, or less where eps would leave 32 bits; what of eps is lost is nothing beside the squares then.
+                    const int up = min(127 - (int)(__float_as_uint(most) >> 23), eps > 0.f ? 50 - ((int)(__float_as_uint(eps) >> 23) - 127) / 2 : 120);
+                    const float part = __uint_as_float((uint32_t)(127 + up / 2) << 23), rest = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
+                    eps = eps * part * part * rest * rest;  // (2^up in two factors)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < E; ++i) x[h][i] = (x[h][i] * part) * rest;
-                ss = squares();
+                        for (int i = 0; i < E; ++i) x[h][i] = (x[h][i] * part) * rest;
+                    ss = squares();
+                }
             }
             const Two8 m = sum_of(ss.h * (1.f / HD), eps);  // (HD is a power of two)
             const float ml = fmaf(ss.l, 1.f / HD, m.l);
@@ -244,7 +254,7 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
         }
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
-    return exponent_byte(top);
+    return exponent_byte(top) + (ANY && far ? FAR_ROW : 0);
 }
 // A key by eight lanes, as bytes: of any size, in 64 bits, a number after the other.
 template <int HD, typename TW>
@@ -284,7 +294,7 @@ __device__ __noinline__ int far_bytes(const Norm8& a, const __nv_bfloat16* row, 
         }
         const float f = to_be_rounded(x);
         if (i < 2 * E) top = fmaxf(top, finite_abs(f));
-        else reinterpret_cast<unsigned char*>(four)[i - 2 * E] = (unsigned char)pack2(f * back, 0.f);
+        else reinterpret_cast<unsigned char*>(four)[i - 2 * E] = (unsigned char)far_pair(pack2(f * back, 0.f));
     }
     return b;
 }
@@ -292,7 +302,19 @@ __device__ __noinline__ int far_bytes(const Norm8& a, const __nv_bfloat16* row, 
 template <int HD, typename TW>
 __device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, bool far, int pos, int sub, unsigned mask, uint32_t* four) {
     constexpr int E = HD / 16;
-    if (far) return far_bytes<HD, TW>(a, row, pos, sub, mask, four);
+    if (far) {  // it may be
+        float most = 0.f;
+        bool numbers = true;
+#pragma unroll 1
+        for (int i = 0; i < 2 * E; ++i) {
+            const float v = fabsf(__bfloat162float(row[(i < E ? i : HD / 2 - E + i) + sub * E]));
+            most = fmaxf(most, v);
+            numbers &= v < INFINITY;
+        }
+        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
+        if (!__all_sync(mask, numbers) || most >= LARGE_ROW || (most > 0.f && most < SMALL_ROW && a.eps < SMALL_EPS))
+            return far_bytes<HD, TW>(a, row, pos, sub, mask, four);
+    }
     float x[2][E];
     const int b = careful_row<HD, 8, TW>(a, row, is_v, pos, sub, mask, x);
     const float back = power_back(b);
@@ -344,7 +366,7 @@ __device__ __forceinline__ int make_bytes(const Norm8& a, const float (&x)[HD / 
     const float back = power_back(b);
     // a row whose maximum is 0 or not to be trusted: it holds an infinity or NaN and is normed, its squares leave 32 bits (zeros come of it; or, with next
     // to no eps, lost bits), or its rotation does
-    const bool far = !is_v && (top >= 0x1p127f || (a.use_norm && (top == 0.f || a.eps < 0x1p-60f)));  // (the same for the lanes of the row)
+    const bool far = !is_v && (top >= 0x1p127f || (a.use_norm && (top == 0.f || a.eps < SMALL_EPS)));  // (the same for the lanes of the row)
     bool care = far || top == INFINITY;
     if (is_v || !(a.use_norm || turns)) {
 #pragma unroll

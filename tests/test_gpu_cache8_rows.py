@@ -204,3 +204,36 @@ def test_a_layer_whose_norm_weights_begin_anywhere(d):
             got.append(F().attention_decode8(q, kv, kv_len, slots, 70, d**-0.5))
     F().check_kernel_errors(DEV)
     assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_the_decode_kernel_writes_the_same_bytes(d, eps):
+    """Rows of zeros, of zeros but for a number, of far and ordinary sizes, of infinities and NaN, with and without signs: as the write by itself."""
+    n, n_q, n_kv = 12, 2, 2
+    keys = rand(n, n_kv, d, seed=1)
+    keys[0] = 0
+    keys[1] = -0.0
+    keys[2, :, 1:] = 0
+    keys[3, :, ::2] = -0.0
+    for i, power in enumerate((-100, -65, 62, 64, 100)):
+        keys[4 + i] *= 2.0**power
+        keys[4 + i, :, ::3] = -0.0
+    keys[9, 0, 5], keys[9, 1, 7] = float("inf"), float("nan")
+    keys[10, :, 3] = 2.0**70
+    keys[11] *= 2.0**-24
+    qkv = torch.cat([rand(n, n_q, d, seed=2), keys, rand(n, n_kv, d, seed=3)], 1).to(torch.bfloat16).view(n, -1).to(DEV)
+    w = (1 + 0.1 * rand(d, seed=4)).float()
+    w[::5] *= -1
+    cos, sin = (t.to(DEV) for t in tables(40, d))
+    positions, pages = [3 * i for i in range(n)], []
+    for fused in (True, False):
+        kv, slots, _ = empty_pages(n, 40, n_kv, d)
+        how = (w.to(DEV), w.to(DEV), eps, cos, sin)
+        if fused:
+            F().attention_decode8_fused(qkv, n_q, n_kv, d, *how, kv, ints(*[p + 1 for p in positions]), slots, max(positions), 40, 0.1)
+        else:
+            F().qk_norm_rope_write8(qkv, n_q, n_kv, d, *how, ints(*positions), ints(*range(n)), slots, kv, max(positions))
+        pages.append(kv)
+    for name in ("k", "v", "k_exp", "v_exp"):
+        assert torch.equal(getattr(pages[0], name).view(torch.uint8), getattr(pages[1], name).view(torch.uint8)), name
