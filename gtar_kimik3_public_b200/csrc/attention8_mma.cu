@@ -529,6 +529,9 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
                         if (none >> mine & 1) s[h][n][i] = NAN;
                         if (key > top || (a.window > 0 && key <= top - a.window)) s[h][n][i] = -INFINITY;
                     }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // (places that no row sees hold any power: theirs is not to look small)
+                if (key0 + 4 * g + i >= u.end || key0 + 4 * g + i < begin) ev[i] = 4096.f;
         }
         bool beyond = false;
 #pragma unroll

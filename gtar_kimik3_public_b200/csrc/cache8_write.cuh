@@ -138,9 +138,9 @@ __device__ __forceinline__ float to_be_rounded(float high, float low) {
 }
 
 constexpr float LARGEST = 3.402823466e38f;
-// The squares of a row whose largest number is below SMALL_ROW end at 2^-149 with bits that count, where eps does not outweigh them; below LARGE_ROW no sum of
-// squares leaves 32 bits.
-constexpr float SMALL_EPS = 0x1p-60f, SMALL_ROW = 0x1p-26f, LARGE_ROW = 0x1p60f;
+// Squares whose sum is below SMALL_SQUARES end at 2^-149 with bits that count, where eps does not outweigh them; below LARGE_ROW no sum of squares leaves
+// 32 bits.
+constexpr float SMALL_EPS = 0x1p-60f, SMALL_SQUARES = 0x1p-52f, LARGE_ROW = 0x1p60f;
 
 // A key, or a row of values as it is, by LANES lanes that have HD / 2 / LANES neighbouring numbers of each half: the numbers to be rounded; the byte of the
 // row's power comes back.  By a whole warp rows of any size (FAR_ROW is added where squares had left 32 bits); by fewer lanes (where the registers that this
@@ -162,12 +162,17 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
     }
     if (!is_v) {
         if (a.use_norm) {
-            const auto squares = [&] {
-                Two8 ss = {0.f, 0.f};
+            Two8 ss;
+            float eps = a.eps;
+            // (once, but for rows whose squares leave 32 bits: these a second time, the row times a power of two and eps times its square, which comes to
+            // the same; the same code again, for a second sum of its own costs decode steps of 64 sequences 2%)
+#pragma unroll 1
+            for (;;) {
+                ss = {0.f, 0.f};
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < E; ++i) {  // (the square of a bfloat16 number is exact, where it is one of 32 bits)
+                    for (int i = 0; i < E; ++i) {  // (the square of a bfloat16 number is exact)
                         const Two8 t = sum_of(ss.h, __fmul_rn(x[h][i], x[h][i]));
                         ss = {t.h, __fadd_rn(ss.l, t.l)};
                     }
@@ -177,32 +182,16 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
                     const Two8 t = sum_of(ss.h, oh);
                     ss = {t.h, __fadd_rn(t.l, __fadd_rn(ss.l, ol))};
                 }
-                return ss;
-            };
-            Two8 ss = squares();
-            float eps = a.eps;
-            if (ANY && (!(ss.h < INFINITY) || eps < SMALL_EPS)) {  // (the same for the lanes of the row)
-                float most = 0.f;
+                if (!ANY || far || (ss.h < INFINITY && (eps >= SMALL_EPS || ss.h >= SMALL_SQUARES))) break;  // (the same for the lanes of the row)
+                const float by = ss.h < INFINITY ? 0x1p70f : 0x1p-70f;
+                far = true;
+                eps = eps * by * by;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < E; ++i) most = fmaxf(most, finite_abs(x[h][i]));
-#pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
-                far = !(ss.h < INFINITY) || (most > 0.f && most < SMALL_ROW);
-                if (far) {
-                    // Squares that leave 32 bits: the row times a power of two, and eps times its square, come to the same.  The row's largest finite number
-                    // becomes one of 1 to 2, or less where eps would leave 32 bits; what of eps is lost is nothing beside the squares then.
-                    const int up = min(127 - (int)(__float_as_uint(most) >> 23), eps > 0.f ? 50 - ((int)(__float_as_uint(eps) >> 23) - 127) / 2 : 120);
-                    const float part = __uint_as_float((uint32_t)(127 + up / 2) << 23), rest = __uint_as_float((uint32_t)(127 + up - up / 2) << 23);
-                    eps = eps * part * part * rest * rest;  // (2^up in two factors)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < E; ++i) x[h][i] = (x[h][i] * part) * rest;
-                    ss = squares();
-                }
+                    for (int i = 0; i < E; ++i) x[h][i] *= by;
             }
+            far = far && ss.h != 0.f;  // (a row of zeros is an ordinary one)
             const Two8 m = sum_of(ss.h * (1.f / HD), eps);  // (HD is a power of two)
             const float ml = fmaf(ss.l, 1.f / HD, m.l);
             float r = rsqrtf(m.h), dr = 0.f;
@@ -227,6 +216,7 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
             float c[E], sn[E];
             load_run<E>(a.cos_table + (size_t)pos * HALF + sub * E, c);
             load_run<E>(a.sin_table + (size_t)pos * HALF + sub * E, sn);
+            float most = 0.f;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const float u = x[0][i], v = x[1][i], ul = low[0][i], vl = low[1][i];
@@ -236,11 +226,21 @@ __device__ __forceinline__ int careful_row(const Norm8& a, const __nv_bfloat16* 
                     const Two8 p = product_of(h ? v : u, c[i]), q = product_of(h ? u : v, s), t = sum_of(p.h, q.h);
                     x[h][i] = t.h;
                     low[h][i] = __fadd_rn(__fadd_rn(t.l, __fadd_rn(p.l, q.l)), __fmaf_rn(h ? vl : ul, c[i], __fmul_rn(h ? ul : vl, s)));
-                    if (ANY && fabsf(t.h) == INFINITY && fabsf(u) < INFINITY && fabsf(v) < INFINITY) {  // of finite numbers: the largest that there is
-                        x[h][i] = copysignf(LARGEST, t.h);
-                        low[h][i] = 0.f;
-                    }
+                    most = fmaxf(most, fabsf(t.h));
                 }
+            }
+            if (ANY && !a.use_norm && __builtin_expect(most == INFINITY, 0)) {  // more than 32 bits hold: of finite numbers the largest that there is
+                float u[E], v[E];
+                load_run<E>(row + sub * E, u);
+                load_run<E>(row + HALF + sub * E, v);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (fabsf(x[h][i]) == INFINITY && fabsf(u[i]) < INFINITY && fabsf(v[i]) < INFINITY) {
+                            x[h][i] = copysignf(LARGEST, x[h][i]);
+                            low[h][i] = 0.f;
+                        }
             }
         }
     }
@@ -303,16 +303,20 @@ template <int HD, typename TW>
 __device__ __noinline__ int careful_bytes(const Norm8& a, const __nv_bfloat16* row, bool is_v, bool far, int pos, int sub, unsigned mask, uint32_t* four) {
     constexpr int E = HD / 16;
     if (far) {  // it may be
-        float most = 0.f;
+        float most = 0.f, ss = 0.f;
         bool numbers = true;
 #pragma unroll 1
         for (int i = 0; i < 2 * E; ++i) {
             const float v = fabsf(__bfloat162float(row[(i < E ? i : HD / 2 - E + i) + sub * E]));
             most = fmaxf(most, v);
+            ss += v * v;
             numbers &= v < INFINITY;
         }
-        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
-        if (!__all_sync(mask, numbers) || most >= LARGE_ROW || (most > 0.f && most < SMALL_ROW && a.eps < SMALL_EPS))
+        for (int o = 1; o < 8; o <<= 1) {
+            most = fmaxf(most, __shfl_xor_sync(mask, most, o));
+            ss += __shfl_xor_sync(mask, ss, o);
+        }
+        if (!__all_sync(mask, numbers) || most >= LARGE_ROW || (most > 0.f && ss < SMALL_SQUARES && a.eps < SMALL_EPS))
             return far_bytes<HD, TW>(a, row, pos, sub, mask, four);
     }
     float x[2][E];

@@ -21,9 +21,9 @@ def lone(n, n_kv, d, power, at, seed=2):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("n_q,n_kv", [(4, 2), (16, 1)])
-@pytest.mark.parametrize("cut", [None, (1, 0), (4, 0), (0, 40)])
-@pytest.mark.parametrize("power", [12, 24, 40, 100])
-@pytest.mark.parametrize("n,at", [(300, 3), (300, 290), (3000, 1500)])
+@pytest.mark.parametrize("cut", [(1, 0), (4, 0), (0, 40)])
+@pytest.mark.parametrize("power", [12, 24, 100])
+@pytest.mark.parametrize("n,at", [(300, 3), (300, 290), (1500, 700)])
 def test_decode(d, n_q, n_kv, cut, power, n, at):
     kv, slots, table = empty_pages(1, n, n_kv, d)
     fill(kv, table, int(slots[0]), rand(n, n_kv, d, seed=1), lone(n, n_kv, d, power, at))
@@ -36,8 +36,8 @@ def test_decode(d, n_q, n_kv, cut, power, n, at):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("few", [True, False])
 @pytest.mark.parametrize("window", [0, 200])
-@pytest.mark.parametrize("power", [12, 24, 40, 100])
-@pytest.mark.parametrize("at", [3, 150, 296])
+@pytest.mark.parametrize("power", [12, 24, 100])
+@pytest.mark.parametrize("at", [3, 296])
 def test_several_tokens(d, few, window, power, at, monkeypatch):
     monkeypatch.setattr(F(), "rows8_wins", lambda *sizes: few)
     n, m, n_q, n_kv = 300, 7, 8, 2
