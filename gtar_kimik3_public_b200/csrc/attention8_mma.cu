@@ -12,8 +12,9 @@
 //     o8 = sum_j 2^(s_j + ev_j - B) v8_j   B near the largest s_j + ev_j    out = o8 2^(B - A) / l
 // A and B are moved only when a number would pass 2^14 or 2^15 (halves end at 65,504): after a sequence's first keys hardly ever, and then no lane
 // has to ask the others for a maximum.  B is set 7 below the largest, so that probabilities keep all their bits down to 2^-21 of it.  Where a tile's
-// values are more than 2^7 smaller than those that B goes by (a column in which the large ones have nothing would show what is lost), what the halves of
-// probabilities above 2^-32 leave over is added by itself.  (To look for such tiles costs 64 sequences of 1,024 to 8,192 tokens 0.4 of 101 us.)
+// values are more than 2^9 smaller than those that B goes by (a column in which the large ones have nothing would show what is lost), what the halves of
+// probabilities above 2^-32 leave over is added by itself.  (To look for such tiles, none of which random keys and values have, costs 64 sequences of
+// 1,024 to 8,192 tokens 0.4 of 101 us, one of 131,072 tokens 1.6 of 55, sixteen times four tokens 0.9 of 27.)
 //
 // The contraction over d may take d in any order that both operands share, and the keys of a product any order that P and V share: lane (g, t) =
 // (lane / 4, lane % 4) reads sixteen bytes in one piece of the keys 4g .. 4g + 3, and of the values 8t .. 8t + 7 its own sixteen (or eight) columns,
@@ -454,7 +455,7 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
 #pragma unroll
     for (int i = 0; i < 8; ++i) v_at[i] = At::value(8 * t + i, D / 8 * g);
     uint32_t place = ring;
-    float gap = -INFINITY;  // the largest B - A of this lane's rows
+    float gap = -INFINITY;  // the largest B - A - 2 of this lane's rows
 #pragma unroll 1
     for (; at < tile_end; at += WARPS) {
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -579,7 +580,7 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
                         }
                         ref_a[n][i] = na;
                         ref_b[n][i] = nb;
-                        if (na > NONE) gap = fmaxf(gap, nb - na);
+                        if (na > NONE) gap = fmaxf(gap, nb - na - 2.f);
                     }
             }
             if (__builtin_expect(__any_sync(0xffffffffu, least < gap), 0)) {
@@ -611,7 +612,8 @@ __device__ __forceinline__ void piece(const GkPages8& p, const Rows8& a, const F
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int mine = 2 * h + (i & 1) * 4 + (i >> 1);
-                            v[i] = none >> (8 * t + mine) & 1 ? 0u : read_word(place + (h ? v_at[2 + (i & 1) * 4 + (i >> 1)] : v_at[(i & 1) * 4 + (i >> 1)]) + 4 * w);
+                            v[i] = read_word(place + (h ? v_at[2 + (i & 1) * 4 + (i >> 1)] : v_at[(i & 1) * 4 + (i >> 1)]) + 4 * w);
+                            if (none >> (8 * t + mine) & 1) v[i] = 0u;
                         }
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
