@@ -4,8 +4,8 @@
 // rotation (src/layers/rope.py:17-33), order of src/layers/attention.py:82-89.  Queries are 32-bit up to the one rounding to their type, values are only
 // rounded.  Keys come out as the formula in 64 bits (or, in the wide kernels, some 45) rounded once: e4m3's steps are so coarse that a number 2^-22 beside the
 // middle between two of them goes wrong by a sixteenth of itself, which 32 bits do to some three in a million.  The wide kernels make a key in 32
-// bits and do it over where a number or its maximum lies next to a border, one row in some fifty (7,921 tokens of 32/8 heads of 128: 49 us; with
-// every key in 64 bits 114).
+// bits and do it over where a number or its maximum lies next to a border, one row in some fifty (7,921 tokens of 32/8 heads of 128: 52 us; with
+// every key in 64 bits 114), and in 64 bits where its squares leave 32.
 
 #include "cache8_write.cuh"
 

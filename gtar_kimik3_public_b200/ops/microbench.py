@@ -10,8 +10,8 @@
 Each run launches the kernel on fresh inputs (a ring of operand sets larger than the L2 cache, so
 that every launch reads from HBM), times it with CUDA events over a graph replay, and prints one
 JSON line with microseconds per launch, the bytes or flops the kernel has to move or do, and the
-rate they amount to.  The same command line under ``ncu -k regex:<kernel> -c 3`` gives a profile of
-exactly that kernel on a case of a few hundred megabytes.
+rate they amount to.  The same command line under ``ncu --clock-control none -k regex:<kernel> -c 3``, after it has
+run without, gives a profile of exactly that kernel on a case of a few hundred megabytes.
 """
 
 from __future__ import annotations
@@ -140,8 +140,8 @@ def bench_attention_prefill(args) -> dict:
 
 def bench_step(args) -> dict:
     """One decode step of a random model of the Qwen3-0.6B layer sizes, launched kernel by kernel (no
-    graph) between cudaProfilerStart/Stop, so that ``ncu --profile-from-start off`` lists exactly
-    the step's launches."""
+    graph) between cudaProfilerStart/Stop, so that ``ncu --clock-control none
+    --profile-from-start off`` lists exactly the step's launches."""
     import tempfile
 
     from ..engine import Engine, StepEntry
